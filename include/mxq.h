@@ -325,6 +325,55 @@ int64_t mxq_gemm_workspace_bytes(int64_t batch, int64_t M, int64_t N, int64_t K,
 #define MXQ_GEMM_PLAN_ONE_STEP 3
 int mxq_gemm_plan(int64_t batch, int64_t M, int64_t N, int64_t K, int a_kind);
 
+/* ---- a paged key / value cache held in MXFP4 (no counterpart in the reference) -------------------
+ * The cache is num_pages x heads records of page_size * NB * 34 bytes, NB = ceil(head_dim / 32), 16-byte
+ * aligned; page_size a multiple of 16, head_dim 1 to 256.  A record holds, for its page's tokens,
+ *   K codes [page_size][16 NB] | V codes [page_size / 4][16][NB][4] | K scales [page_size][NB] |
+ *   V scales [page_size / 4][NB][4]
+ * e2m1 nibbles with one E8M0 byte for 32 elements (zeros behind head_dim): K rows as mxq_pack_mx writes
+ * them (MXQ_FLAG_PACK_NIBBLES); byte (i, b, t) of a V group of four tokens holds the elements 32 b + 2 i (low
+ * nibble) and 32 b + 2 i + 1 of token t.  A slot is page * page_size + place in the page.  Indexes that the
+ * host cannot see (slots, table entries, lengths, starts) are checked by the kernels: a slot or page outside the
+ * cache is not touched. */
+
+/* Block tables and slots of a step from the requests' lengths.  Request r holds context_lens[r] tokens in the
+ * pages of row r of block_table (width entries, rows table_stride apart) and gets new_lens[r] more (negative
+ * counts as zero).  Pages it lacks come from free_pages[free_start[0]..], in the order of the requests, and are
+ * written to the table; free_next[0] is where the next call starts (beyond free_count: the list ran out, and
+ * the entries that got no page are -1).  starts (requests + 1): exclusive sums of the new lengths, at most
+ * `tokens`; seq_lens: lengths with the new tokens.  For each of `tokens` rows: its slot, its position in the
+ * request and the request it belongs to, or -1 (rows behind the last request; tokens without a page have slot -1).
+ * Repeating a call with the same inputs gives the same results. */
+int mxq_kv_block_tables(const int* context_lens, const int* new_lens, int* block_table, int64_t table_stride, int64_t width,
+                        const int* free_pages, int64_t free_count, const int* free_start, int64_t requests, int page_size,
+                        int64_t tokens, int64_t* slots, int* positions, int* owners, int* starts, int* seq_lens,
+                        int* free_next, void* hip_stream);
+/* Rows k, v (tokens, heads, head_dim; strides in elements, elements of a row contiguous) quantized along
+ * head_dim in blocks of 32 exactly as mxq_pack_mx does (parameters as there) and stored at `slots`; rows whose
+ * slot is outside the cache are left out.  No slot may come twice. */
+int mxq_kv_append_mx(const void* k, const void* v, int dtype, int64_t tokens, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots, void* cache, int64_t num_pages,
+                     int heads, int page_size, int head_dim, int scale_bits, int flush_fp32_subnorms, int rmode, int flags,
+                     void* hip_stream);
+/* The values stored at `slots`, as (tokens, heads, head_dim) of `dtype`; zeros for slots outside the cache. */
+int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* slots, const void* cache, int64_t num_pages,
+                   int heads, int page_size, int head_dim, void* hip_stream);
+/* Attention of rows q (rows, q_heads, head_dim; bf16 or fp16) over the cached tokens of their requests:
+ * out = softmax(scale * q K^T) V, lse = log of the sum of exponentials (may be NULL).  Query head h reads kv head
+ * h / (q_heads / heads).  Request r's rows are starts[r] .. starts[r + 1] - 1 (starts NULL: row r), the last of its
+ * seq_lens[r] tokens; with causal a row sees the tokens up to its own.  Tokens on pages that do not exist are not
+ * seen; a row that sees nothing gets zeros and lse -inf.  Rows behind the last request are left as they are, or
+ * zeroed (lse -inf) with zero_tail.  max_new: the most rows of a request, a hint that only steers the choice of
+ * kernels.  workspace: mxq_kv_attention_workspace_bytes(...) bytes, 8-byte aligned. */
+int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
+                        int64_t out_head_stride, float* lse, int dtype, int64_t rows, int q_heads, const int* block_table,
+                        int64_t table_stride, int64_t width, const int* seq_lens, const int* starts, int64_t requests,
+                        float scale, int causal, int64_t max_new, int zero_tail, const void* cache, int64_t num_pages,
+                        int heads, int page_size, int head_dim, void* workspace, int64_t workspace_bytes, void* hip_stream);
+int64_t mxq_kv_attention_workspace_bytes(int64_t requests, int64_t rows, int q_heads, int64_t max_new, int64_t width, int heads,
+                                         int page_size, int head_dim);
+
+
 /* ---- libmxq_host.so: the same arithmetic compiled for the host ----------------------------------
  * quantize_mx_func_cpp (mx/cpp/funcs.cpp:23-98) and quantize_elemwise_func_cpp
  * (mx/cpp/funcs.cpp:117-149) take CPU tensors; these are their stand-ins.  Pointers are host

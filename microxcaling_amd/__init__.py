@@ -18,3 +18,4 @@ from .layernorm import LayerNorm, RMSNorm, layer_norm
 from .activations import (sigmoid, tanh, relu, relu6, leaky_relu, silu, gelu,
                           Sigmoid, Tanh, ReLU, ReLU6, LeakyReLU, SiLU, GELU)
 from .convolution import Conv1d, Conv2d, Conv3d, conv1d, conv2d, conv3d
+from .kv_cache import PackedKVCache, new_kv_cache, kv_block_tables, kv_append, kv_read, kv_attention

@@ -59,7 +59,7 @@ def _run(cmd, verbose):
 
 
 GPU_SOURCES = ["mxq_capi.hip", "mxq_capi_gemm.hip", "mxq_capi_chain.hip", "mxq_capi_norm.hip",
-               "mxq_capi_scores.hip"]
+               "mxq_capi_scores.hip", "mxq_capi_kv.hip", "mxq_capi_kv_decode.hip", "mxq_capi_kv_prompt.hip"]
 
 
 def build_gpu(verbose=True):

@@ -1,0 +1,252 @@
+// C ABI of libmxq_gfx950.so, continued: the paged MXFP4 key / value cache.
+#include "mxq_capi_kv.h"
+#include "mxq_kv_rows.h"
+
+namespace mxq_kv {
+void launch_decode(int dtype, const void* args, const Plan& p, hipStream_t s);
+void launch_prompt(int dtype, const void* args, const Plan& p, hipStream_t s);
+}  // namespace mxq_kv
+
+namespace {
+
+using mxq_kv::Plan;
+
+// tokens that a table row may name: positions stay far from the end of int32
+constexpr int64_t kMaxTokens = (int64_t)1 << 30;
+
+int make_cache(void* data, int64_t num_pages, int heads, int page_size, int head_dim, KvCache* c, const char* who) {
+    if (head_dim < 1 || head_dim > 32 * KV_MAX_NB)
+        return fail(MXQ_ERR_ARGUMENT, "%s: head_dim must be 1 to %d, got %d", who, 32 * KV_MAX_NB, head_dim);
+    if (page_size < 16 || page_size % 16 != 0 || page_size > 65536)
+        return fail(MXQ_ERR_ARGUMENT, "%s: page_size must be a multiple of 16 up to 65536, got %d", who, page_size);
+    if (heads < 1 || heads > 65535) return fail(MXQ_ERR_ARGUMENT, "%s: bad number of heads %d", who, heads);
+    if (num_pages < 1 || num_pages > 0x7FFFFFFF) return fail(MXQ_ERR_ARGUMENT, "%s: the cache has no pages, or too many", who);
+    if (!data) return fail(MXQ_ERR_ARGUMENT, "%s: null pointer", who);
+    if (!aligned16(data)) return fail(MXQ_ERR_ARGUMENT, "%s: the cache must be 16-byte aligned", who);
+    c->data = reinterpret_cast<unsigned char*>(data);
+    c->num_pages = num_pages;
+    c->heads = heads;
+    c->page_size = page_size;
+    c->head_dim = head_dim;
+    c->nb = (head_dim + 31) / 32;
+    c->record = (int64_t)page_size * c->nb * KV_TOKEN_BYTES;
+    int64_t total;
+    if (mul_overflows(num_pages, heads, c->record, &total)) return fail(MXQ_ERR_ARGUMENT, "%s: size overflows int64", who);
+    return MXQ_OK;
+}
+
+template <int DT, int RMODE, bool ZE, bool LEAN>
+struct LaunchAppend {
+    static void run(KvRowsArgs a, MxParams p, uint32_t max_code, int grid, hipStream_t s) {
+        if constexpr (!ZE) {
+            if (max_code != 0u) {
+                kv_append_kernel<DT, RMODE, ZE, true><<<grid, kThreads, 0, s>>>(a, p, max_code);
+                return;
+            }
+        }
+        kv_append_kernel<DT, RMODE, ZE, false><<<grid, kThreads, 0, s>>>(a, p, 0u);
+    }
+};
+
+// Which kernels a call runs, and with what shares.  max_new: tokens that a request brings at most (a hint: every
+// choice made with it is right for any number).
+Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64_t room, int heads, int nb) {
+    Plan p;
+    p.nb = nb;
+    if (max_new > rows) max_new = rows;
+    if (max_new < 1) max_new = 1;
+    const int64_t columns = max_new * group;
+    p.prompt = columns > 64;
+    p.decode = true;
+    p.decode_columns = p.prompt ? 64 : 0x7FFFFFFF;
+    p.ct = columns <= 16 ? 1 : 2;
+    const int64_t units = ceil_div(room, KV_UNIT) > 0 ? ceil_div(room, KV_UNIT) : 1;
+    p.decode_items = rows * group / (16 * p.ct) + requests;
+    p.whole = units <= 4;
+    const int64_t chip = 256 * (p.ct == 1 ? 4 : 3);
+    p.shares = ceil_div(chip, heads);
+    if (p.shares > p.decode_items * units) p.shares = p.decode_items * units;
+    const int64_t cols = 64 * kv_prompt_ct(nb);
+    p.prompt_tiles = rows * group / cols + requests;
+    return p;
+}
+
+int64_t part_bytes(const Plan& p, int heads) {
+    return p.whole ? 0 : p.shares * heads * 2 * (16 * p.ct) * (32 * p.nb + 2) * (int64_t)sizeof(float);
+}
+
+}  // namespace
+
+#pragma GCC visibility push(default)
+extern "C" {
+
+int mxq_kv_block_tables(const int* context_lens, const int* new_lens, int* block_table, int64_t table_stride, int64_t width,
+                        const int* free_pages, int64_t free_count, const int* free_start, int64_t requests, int page_size,
+                        int64_t tokens, int64_t* slots, int* positions, int* owners, int* starts, int* seq_lens,
+                        int* free_next, void* hip_stream) {
+    const char* who = "mxq_kv_block_tables";
+    if (requests < 0 || width < 0 || free_count < 0 || tokens < 0) return fail(MXQ_ERR_ARGUMENT, "%s: negative size", who);
+    if (page_size < 16 || page_size % 16 != 0 || page_size > 65536)
+        return fail(MXQ_ERR_ARGUMENT, "%s: page_size must be a multiple of 16 up to 65536, got %d", who, page_size);
+    if (requests > 0x7FFFFF00 || tokens > 0x7FFFFF00) return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
+    if (width * page_size > kMaxTokens) return fail(MXQ_ERR_ARGUMENT, "%s: a table row names too many tokens", who);
+    if (requests > 0 && (!context_lens || !new_lens || !seq_lens || (width > 0 && !block_table)))
+        return fail(MXQ_ERR_ARGUMENT, "%s: null pointer", who);
+    if ((free_count > 0 && !free_pages) || !free_start || !free_next || !starts ||
+        (tokens > 0 && (!slots || !positions || !owners)))
+        return fail(MXQ_ERR_ARGUMENT, "%s: null pointer", who);
+    KvTablesArgs a;
+    a.context = context_lens;
+    a.fresh = new_lens;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.width = (int)width;
+    a.free_pages = free_pages;
+    a.free_count = free_count;
+    a.free_start = free_start;
+    a.requests = (int)requests;
+    a.page_size = page_size;
+    a.tokens = tokens;
+    a.slots = slots;
+    a.positions = positions;
+    a.owners = owners;
+    a.starts = starts;
+    a.seq_lens = seq_lens;
+    a.free_next = free_next;
+    const int64_t grid = ceil_div(tokens, KV_TABLE_TOKENS) > 0 ? ceil_div(tokens, KV_TABLE_TOKENS) : 1;
+    kv_block_tables_kernel<KV_TABLE_TOKENS><<<(unsigned)grid, kThreads, 0, (hipStream_t)hip_stream>>>(a);
+    return check_launch(who);
+}
+
+int mxq_kv_append_mx(const void* k, const void* v, int dtype, int64_t tokens, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots, void* cache, int64_t num_pages,
+                     int heads, int page_size, int head_dim, int scale_bits, int flush_fp32_subnorms, int rmode, int flags,
+                     void* hip_stream) {
+    const char* who = "mxq_kv_append_mx";
+    if (f16_ops(dtype, flags))
+        return fail(MXQ_ERR_ARGUMENT, "%s: fp16 tensors have a packed form under MXQ_FLAG_EXACT_EXPONENT only "
+                    "(the op-by-op fp16 arithmetic of the default mode has no packing kernel)", who);
+    MxParams p;
+    bool ze;
+    int rc = make_mx_params(dtype, scale_bits, 2, 3, 6.0f, flush_fp32_subnorms, rmode, flags, &p, &ze, who);
+    if (rc) return rc;
+    KvRowsArgs a;
+    rc = make_cache(cache, num_pages, heads, page_size, head_dim, &a.c, who);
+    if (rc) return rc;
+    if (tokens < 0) return fail(MXQ_ERR_ARGUMENT, "%s: negative size", who);
+    if (tokens == 0) return MXQ_OK;
+    if (!k || !v || !slots) return fail(MXQ_ERR_ARGUMENT, "%s: null pointer", who);
+    a.k = k;
+    a.v = v;
+    a.k_token = k_token_stride;
+    a.k_head = k_head_stride;
+    a.v_token = v_token_stride;
+    a.v_head = v_head_stride;
+    a.slots = slots;
+    a.tokens = tokens;
+    const int per16 = 16 / elem_size(dtype);             // elements in 16 bytes
+    a.wide = aligned16(k) && aligned16(v) && head_dim % 8 == 0 && k_token_stride % per16 == 0 && k_head_stride % per16 == 0 &&
+             v_token_stride % per16 == 0 && v_head_stride % per16 == 0;
+    const int64_t items = (tokens + 3) / 4 * heads * a.c.nb * 2;
+    dispatch<LaunchAppend>(dtype, rmode, ze, true, a, p, mxq_max_code(p.fmt), grid_for(ceil_div(items, kThreads / 16)),
+                           (hipStream_t)hip_stream);
+    return check_launch(who);
+}
+
+int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* slots, const void* cache, int64_t num_pages,
+                   int heads, int page_size, int head_dim, void* hip_stream) {
+    const char* who = "mxq_kv_read_mx";
+    if (dtype < 0 || dtype > 2) return fail(MXQ_ERR_ARGUMENT, "%s: unknown dtype code %d", who, dtype);
+    KvReadArgs a;
+    int rc = make_cache(const_cast<void*>(cache), num_pages, heads, page_size, head_dim, &a.c, who);
+    if (rc) return rc;
+    if (tokens < 0) return fail(MXQ_ERR_ARGUMENT, "%s: negative size", who);
+    if (tokens == 0) return MXQ_OK;
+    if (!k || !v || !slots) return fail(MXQ_ERR_ARGUMENT, "%s: null pointer", who);
+    a.k = k;
+    a.v = v;
+    a.slots = slots;
+    a.tokens = tokens;
+    const int wide = aligned16(k) && aligned16(v) && head_dim % 8 == 0;
+    const int64_t items = (tokens + 3) / 4 * heads * a.c.nb * 2;
+    const int grid = grid_for(ceil_div(items, kThreads / 16));
+    hipStream_t s = (hipStream_t)hip_stream;
+    if (dtype == MXQ_DTYPE_F32) kv_read_kernel<MXQ_F32><<<grid, kThreads, 0, s>>>(a, wide);
+    else if (dtype == MXQ_DTYPE_BF16) kv_read_kernel<MXQ_BF16><<<grid, kThreads, 0, s>>>(a, wide);
+    else kv_read_kernel<MXQ_F16><<<grid, kThreads, 0, s>>>(a, wide);
+    return check_launch(who);
+}
+
+int64_t mxq_kv_attention_workspace_bytes(int64_t requests, int64_t rows, int q_heads, int64_t max_new, int64_t width, int heads,
+                                         int page_size, int head_dim) {
+    if (requests <= 0 || rows <= 0 || heads <= 0 || q_heads < heads || width < 0 || page_size <= 0 || head_dim < 1 ||
+        head_dim > 32 * KV_MAX_NB)
+        return 0;
+    return part_bytes(make_plan(requests, rows, q_heads / heads, max_new, width * page_size, heads, (head_dim + 31) / 32), heads);
+}
+
+int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
+                        int64_t out_head_stride, float* lse, int dtype, int64_t rows, int q_heads, const int* block_table,
+                        int64_t table_stride, int64_t width, const int* seq_lens, const int* starts, int64_t requests,
+                        float scale, int causal, int64_t max_new, int zero_tail, const void* cache, int64_t num_pages,
+                        int heads, int page_size, int head_dim, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    const char* who = "mxq_kv_attention_mx";
+    if (dtype != MXQ_DTYPE_BF16 && dtype != MXQ_DTYPE_F16)
+        return fail(MXQ_ERR_ARGUMENT, "%s: queries must be bf16 or fp16 (dtype code %d)", who, dtype);
+    KvAttnArgs a;
+    int rc = make_cache(const_cast<void*>(cache), num_pages, heads, page_size, head_dim, &a.c, who);
+    if (rc) return rc;
+    if (q_heads < 1 || q_heads % heads != 0)
+        return fail(MXQ_ERR_ARGUMENT, "%s: %d query heads do not share %d kv heads evenly", who, q_heads, heads);
+    if (rows < 0 || requests < 0 || width < 0) return fail(MXQ_ERR_ARGUMENT, "%s: negative size", who);
+    if (!(scale > -__builtin_inff() && scale < __builtin_inff())) return fail(MXQ_ERR_ARGUMENT, "%s: scale must be finite", who);
+    if (rows == 0) return MXQ_OK;
+    if (requests == 0 && !starts) return fail(MXQ_ERR_ARGUMENT, "%s: rows without requests", who);
+    if (!starts && rows != requests) return fail(MXQ_ERR_ARGUMENT, "%s: without starts every request has one row", who);
+    if (requests > 0x7FFFFF00 || rows * q_heads > 0x7FFFFF00 || width * page_size > kMaxTokens)
+        return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
+    if (!q || !out || (requests > 0 && (!seq_lens || (width > 0 && !block_table))))
+        return fail(MXQ_ERR_ARGUMENT, "%s: null pointer", who);
+    const Plan p = make_plan(requests, rows, q_heads / heads, max_new, width * page_size, heads, a.c.nb);
+    if (workspace_bytes < part_bytes(p, heads) || (part_bytes(p, heads) > 0 && !workspace))
+        return fail(MXQ_ERR_ARGUMENT, "%s: the workspace is too small", who);
+    if (reinterpret_cast<uintptr_t>(workspace) & 7) return fail(MXQ_ERR_ARGUMENT, "%s: the workspace must be 8-byte aligned", who);
+    a.q = reinterpret_cast<const unsigned short*>(q);
+    a.q_token = q_token_stride;
+    a.q_head = q_head_stride;
+    a.out = reinterpret_cast<unsigned short*>(out);
+    a.out_token = out_token_stride;
+    a.out_head = out_head_stride;
+    a.lse = lse;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.width = (int)width;
+    a.seq_lens = seq_lens;
+    a.starts = starts;
+    a.requests = (int)requests;
+    a.group = q_heads / heads;
+    a.rows = rows;
+    a.scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
+    a.q_sign = scale < 0 ? 0x80008000u : 0u;
+    a.causal = causal ? 1 : 0;
+    a.q_wide = aligned16(q) && head_dim % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
+    a.out_wide = aligned16(out) && head_dim % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0;
+    a.zero_tail = zero_tail ? 1 : 0;
+    a.tile_columns = 16 * p.ct;
+    a.decode_columns = p.decode_columns;
+    a.whole = p.whole ? 1 : 0;
+    a.shares = (int)p.shares;
+    a.part = reinterpret_cast<float*>(workspace);
+    hipStream_t s = (hipStream_t)hip_stream;
+    mxq_kv::launch_decode(dtype, &a, p, s);
+    rc = check_launch(who);
+    if (rc) return rc;
+    if (p.prompt) {
+        mxq_kv::launch_prompt(dtype, &a, p, s);
+        rc = check_launch(who);
+    }
+    return rc;
+}
+
+}  // extern "C"
+#pragma GCC visibility pop

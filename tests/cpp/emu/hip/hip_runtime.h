@@ -327,6 +327,18 @@ inline T __shfl_down(T v, unsigned delta, int width = 64) {
     return emu_shuffle(v, emu::lane_in_wave() + (int)delta);   // past the end of the wave: the lane's own value
 }
 
+template <class T>
+inline T __shfl_up(T v, unsigned delta, int width = 64) {
+    if (width != 64) __builtin_trap();
+    return emu_shuffle(v, emu::lane_in_wave() - (int)delta);   // before the wave's begin: the lane's own value
+}
+// v_readlane_b32: the value of one lane, which every lane names alike
+inline int emu_readlane(int v, int lane) {
+    if (lane < 0 || lane >= emu::kWave) __builtin_trap();
+    return (int)(uint32_t)emu::exchange((uint32_t)v, lane, (uint32_t)v);
+}
+#define __builtin_amdgcn_readlane emu_readlane
+
 inline int __all(int pred) {                               // over the lanes of the wave that are still there
     emu::Block& b = *emu::block();
     const int lane = emu::lane_in_block(), w = lane / emu::kWave;
@@ -384,6 +396,77 @@ inline emu_pair emu_permlane16_swap(unsigned a, unsigned b, bool, bool) {
     return upper ? emu_pair{{got, b}} : emu_pair{{a, got}};
 }
 #define __builtin_amdgcn_permlane16_swap emu_permlane16_swap
+
+// v_permlane32_swap_b32: the first operand of the lanes 32-63 trades places with the second operand of the lanes
+// 0-31 (lane L + 32 with lane L)
+inline emu_pair emu_permlane32_swap(unsigned a, unsigned b, bool, bool) {
+    const int lane = emu::lane_in_wave();
+    const bool upper = (lane & 32) != 0;
+    const uint64_t mine = upper ? a : b;
+    const unsigned got = (unsigned)emu::exchange(mine, upper ? lane - 32 : lane + 32, mine);
+    return upper ? emu_pair{{got, b}} : emu_pair{{a, got}};
+}
+#define __builtin_amdgcn_permlane32_swap emu_permlane32_swap
+
+// v_perm_b32: four bytes picked from the eight of {a, b} (0-3: b, 4-7: a)
+inline unsigned emu_perm(unsigned a, unsigned b, unsigned sel) {
+    const uint64_t both = ((uint64_t)a << 32) | b;
+    unsigned out = 0;
+    for (int i = 0; i < 4; ++i) {
+        const unsigned s = (sel >> (8 * i)) & 255u;
+        if (s > 7) __builtin_trap();
+        out |= (unsigned)((both >> (8 * s)) & 255u) << (8 * i);
+    }
+    return out;
+}
+#define __builtin_amdgcn_perm emu_perm
+
+// v_log_f32 (base 2)
+#define __builtin_amdgcn_logf log2f
+
+// v_cvt_scalef32_pk_bf16_fp4: byte `sel` of the codes as two bf16 values (the low nibble in the low half), times
+// 2^(exponent field of scale - 127); a field of 255 gives NaN
+typedef __bf16 emu_bf16x2 __attribute__((ext_vector_type(2)));
+inline emu_bf16x2 emu_cvt_fp4(unsigned codes, float scale, int sel) {
+    static const float mag[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
+    const int e = (int)((__float_as_uint(scale) >> 23) & 255u);
+    const unsigned byte = (codes >> (8 * sel)) & 255u;
+    uint32_t out = 0;
+    for (int n = 0; n < 2; ++n) {
+        const unsigned c = (byte >> (4 * n)) & 15u;
+        const float v = e == 255 ? NAN : ldexpf((c & 8) ? -mag[c & 7] : mag[c & 7], e - 127);
+        out |= (__float_as_uint(v) >> 16) << (16 * n);       // exact: two significant bits
+    }
+    return __builtin_bit_cast(emu_bf16x2, out);
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4 emu_cvt_fp4
+
+// v_mfma_f32_16x16x32_bf16: lane l supplies row (column) l % 16, K = 8 (l / 16) .. + 7, and receives column l % 16,
+// rows 4 (l / 16) + r
+template <class VB, class VF>
+inline VF emu_mfma_bf16(const VB& a, const VB& b, const VF& c, int, int, int) {
+    emu::Block& blk = *emu::block();
+    const int lane = emu::lane_in_block(), w0 = lane / emu::kWave * emu::kWave, l = lane % emu::kWave;
+    blk.operand[lane][0] = &a;
+    blk.operand[lane][1] = &b;
+    emu::wave_meet();
+    for (int other = w0; other < w0 + emu::kWave; ++other)
+        if (!blk.active[other].load()) __builtin_trap();
+    VF d = c;
+    for (int r = 0; r < 4; ++r) {
+        double sum = (double)c[r];
+        for (int g = 0; g < 4; ++g) {
+            const uint16_t* x = static_cast<const uint16_t*>(blk.operand[w0 + 4 * (l / 16) + r + 16 * g][0]);
+            const uint16_t* y = static_cast<const uint16_t*>(blk.operand[w0 + l % 16 + 16 * g][1]);
+            for (int k = 0; k < 8; ++k)
+                sum += (double)__uint_as_float((uint32_t)x[k] << 16) * (double)__uint_as_float((uint32_t)y[k] << 16);
+        }
+        d[r] = (float)sum;
+    }
+    emu::wave_meet();
+    return d;
+}
+#define __builtin_amdgcn_mfma_f32_16x16x32_bf16 emu_mfma_bf16
 
 // (object-like macros: the kernels pass braced vectors, whose commas a function-like macro would split)
 template <class VI, class VF>
