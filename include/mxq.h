@@ -364,14 +364,14 @@ int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* s
  * seq_lens[r] tokens; with causal a row sees the tokens up to its own.  Tokens on pages that do not exist are not
  * seen; a row that sees nothing gets zeros and lse -inf.  Rows behind the last request are left as they are, or
  * zeroed (lse -inf) with zero_tail.  max_new: the most rows of a request, a hint that only steers the choice of
- * kernels.  workspace: mxq_kv_attention_workspace_bytes(...) bytes, 8-byte aligned. */
+ * kernels.  workspace: mxq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned. */
 int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
                         int64_t out_head_stride, float* lse, int dtype, int64_t rows, int q_heads, const int* block_table,
                         int64_t table_stride, int64_t width, const int* seq_lens, const int* starts, int64_t requests,
                         float scale, int causal, int64_t max_new, int zero_tail, const void* cache, int64_t num_pages,
                         int heads, int page_size, int head_dim, void* workspace, int64_t workspace_bytes, void* hip_stream);
 int64_t mxq_kv_attention_workspace_bytes(int64_t requests, int64_t rows, int q_heads, int64_t max_new, int64_t width, int heads,
-                                         int page_size, int head_dim);
+                                         int page_size, int head_dim, int dtype);
 
 
 /* ---- libmxq_host.so: the same arithmetic compiled for the host ----------------------------------

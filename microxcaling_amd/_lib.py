@@ -70,7 +70,7 @@ GPU_SYMBOLS = {
     "mxq_kv_attention_mx": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_int, _c_i64, _c_int,
                                      _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_f32, _c_int, _c_i64, _c_int,
                                      _c_ptr, _c_i64, _c_int, _c_int, _c_int, _c_ptr, _c_i64, _c_ptr]),
-    "mxq_kv_attention_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int]),
+    "mxq_kv_attention_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int]),
     "mxq_reduce_sum_inner": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr]),
     "mxq_reduce_max_inner": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr]),
     "mxq_reduce_outer_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),

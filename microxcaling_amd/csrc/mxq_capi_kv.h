@@ -12,7 +12,7 @@ struct Plan {
     int decode_columns;
     int64_t decode_items;          // whole: workgroups of a kv head
     int64_t shares;
-    int64_t prompt_tiles;
+    int64_t prompt_items, prompt_shares;
 };
 }  // namespace mxq_kv
 

@@ -5,6 +5,7 @@
 namespace mxq_kv {
 void launch_decode(int dtype, const void* args, const Plan& p, hipStream_t s);
 void launch_prompt(int dtype, const void* args, const Plan& p, hipStream_t s);
+void launch_join(int dtype, const void* args, const Plan& p, hipStream_t s);
 }  // namespace mxq_kv
 
 namespace {
@@ -30,6 +31,10 @@ int make_cache(void* data, int64_t num_pages, int heads, int page_size, int head
     c->head_dim = head_dim;
     c->nb = (head_dim + 31) / 32;
     c->record = (int64_t)page_size * c->nb * KV_TOKEN_BYTES;
+    int log = 0;                                         // multiply instead of dividing by page_size, exact for 32 bits
+    while ((1 << log) < page_size) ++log;
+    c->divide_by = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << log) - page_size)) / page_size + 1);
+    c->shift_by = (uint32_t)(log - 1);
     int64_t total;
     if (mul_overflows(num_pages, heads, c->record, &total)) return fail(MXQ_ERR_ARGUMENT, "%s: size overflows int64", who);
     return MXQ_OK;
@@ -38,19 +43,21 @@ int make_cache(void* data, int64_t num_pages, int heads, int page_size, int head
 template <int DT, int RMODE, bool ZE, bool LEAN>
 struct LaunchAppend {
     static void run(KvRowsArgs a, MxParams p, uint32_t max_code, int grid, hipStream_t s) {
-        if constexpr (!ZE) {
-            if (max_code != 0u) {
-                kv_append_kernel<DT, RMODE, ZE, true><<<grid, kThreads, 0, s>>>(a, p, max_code);
-                return;
-            }
-        }
-        kv_append_kernel<DT, RMODE, ZE, false><<<grid, kThreads, 0, s>>>(a, p, 0u);
+        kv_append_kernel<DT, RMODE, ZE><<<grid, kThreads, 0, s>>>(a, p, max_code);
     }
 };
 
+// workgroups of the row kernels: each has 16 of the units (head, K or V, block) of a group of four tokens and goes through
+// the groups; enough of them to fill the chip
+int rows_grid(const KvCache& c, int64_t tokens) {
+    const int64_t unit_blocks = ceil_div((int64_t)c.heads * 2 * c.nb, 16), quads = ceil_div(tokens, 4);
+    const int64_t most = ceil_div(kMaxBlocks, unit_blocks);
+    return (int)(unit_blocks * (quads < most ? quads : most));
+}
+
 // Which kernels a call runs, and with what shares.  max_new: tokens that a request brings at most (a hint: every
 // choice made with it is right for any number).
-Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64_t room, int heads, int nb) {
+Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64_t room, int heads, int nb, int terms) {
     Plan p;
     p.nb = nb;
     if (max_new > rows) max_new = rows;
@@ -59,20 +66,29 @@ Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64
     p.prompt = columns > 64;
     p.decode = true;
     p.decode_columns = p.prompt ? 64 : 0x7FFFFFFF;
-    p.ct = columns <= 16 ? 1 : 2;
+    p.ct = columns <= 16 ? 1 : kv_decode_most_ct(nb, terms);
     const int64_t units = ceil_div(room, KV_UNIT) > 0 ? ceil_div(room, KV_UNIT) : 1;
     p.decode_items = rows * group / (16 * p.ct) + requests;
     p.whole = units <= 4;
-    const int64_t chip = 256 * (p.ct == 1 ? 4 : 3);
-    p.shares = ceil_div(chip, heads);
+    const int64_t chip = 256 * kv_decode_waves(nb, p.ct, terms);
+    p.shares = ceil_div(chip, heads) < KV_MAX_SHARES ? ceil_div(chip, heads) : KV_MAX_SHARES;
     if (p.shares > p.decode_items * units) p.shares = p.decode_items * units;
-    const int64_t cols = 64 * kv_prompt_ct(nb);
-    p.prompt_tiles = rows * group / cols + requests;
+    const int64_t cols = 64 * kv_prompt_ct(nb, terms);
+    p.prompt_items = rows * group / cols + requests;
+    p.prompt_shares = 256 * (nb <= 4 ? 2 : 1) / heads > 1 ? 256 * (nb <= 4 ? 2 : 1) / heads : 1;
     return p;
 }
 
-int64_t part_bytes(const Plan& p, int heads) {
+// pieces of the workspace, each a multiple of 16 bytes
+int64_t decode_part_bytes(const Plan& p, int heads) {
     return p.whole ? 0 : p.shares * heads * 2 * (16 * p.ct) * (32 * p.nb + 2) * (int64_t)sizeof(float);
+}
+int64_t prompt_part_bytes(const Plan& p, int heads, int terms) {
+    return p.prompt ? p.prompt_shares * heads * 2 * (64 * kv_prompt_ct(p.nb, terms)) * (32 * p.nb + 2) * (int64_t)sizeof(float) : 0;
+}
+int64_t part_bytes(const Plan& p, int heads, int terms, int64_t requests) {
+    return decode_part_bytes(p, heads) + prompt_part_bytes(p, heads, terms) +
+           (p.prompt ? kv_plan_bytes(p.prompt_items, p.prompt_shares, requests) : 0);
 }
 
 }  // namespace
@@ -147,9 +163,7 @@ int mxq_kv_append_mx(const void* k, const void* v, int dtype, int64_t tokens, in
     const int per16 = 16 / elem_size(dtype);             // elements in 16 bytes
     a.wide = aligned16(k) && aligned16(v) && head_dim % 8 == 0 && k_token_stride % per16 == 0 && k_head_stride % per16 == 0 &&
              v_token_stride % per16 == 0 && v_head_stride % per16 == 0;
-    const int64_t items = (tokens + 3) / 4 * heads * a.c.nb * 2;
-    dispatch<LaunchAppend>(dtype, rmode, ze, true, a, p, mxq_max_code(p.fmt), grid_for(ceil_div(items, kThreads / 16)),
-                           (hipStream_t)hip_stream);
+    dispatch<LaunchAppend>(dtype, rmode, ze, true, a, p, mxq_max_code(p.fmt), rows_grid(a.c, tokens), (hipStream_t)hip_stream);
     return check_launch(who);
 }
 
@@ -168,8 +182,7 @@ int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* s
     a.slots = slots;
     a.tokens = tokens;
     const int wide = aligned16(k) && aligned16(v) && head_dim % 8 == 0;
-    const int64_t items = (tokens + 3) / 4 * heads * a.c.nb * 2;
-    const int grid = grid_for(ceil_div(items, kThreads / 16));
+    const int grid = rows_grid(a.c, tokens);
     hipStream_t s = (hipStream_t)hip_stream;
     if (dtype == MXQ_DTYPE_F32) kv_read_kernel<MXQ_F32><<<grid, kThreads, 0, s>>>(a, wide);
     else if (dtype == MXQ_DTYPE_BF16) kv_read_kernel<MXQ_BF16><<<grid, kThreads, 0, s>>>(a, wide);
@@ -178,11 +191,13 @@ int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* s
 }
 
 int64_t mxq_kv_attention_workspace_bytes(int64_t requests, int64_t rows, int q_heads, int64_t max_new, int64_t width, int heads,
-                                         int page_size, int head_dim) {
+                                         int page_size, int head_dim, int dtype) {
     if (requests <= 0 || rows <= 0 || heads <= 0 || q_heads < heads || width < 0 || page_size <= 0 || head_dim < 1 ||
         head_dim > 32 * KV_MAX_NB)
         return 0;
-    return part_bytes(make_plan(requests, rows, q_heads / heads, max_new, width * page_size, heads, (head_dim + 31) / 32), heads);
+    const int terms = dtype == MXQ_DTYPE_F16 ? 2 : 1;
+    return part_bytes(make_plan(requests, rows, q_heads / heads, max_new, width * page_size, heads, (head_dim + 31) / 32, terms),
+                      heads, terms, requests);
 }
 
 int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
@@ -207,10 +222,16 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
         return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
     if (!q || !out || (requests > 0 && (!seq_lens || (width > 0 && !block_table))))
         return fail(MXQ_ERR_ARGUMENT, "%s: null pointer", who);
-    const Plan p = make_plan(requests, rows, q_heads / heads, max_new, width * page_size, heads, a.c.nb);
-    if (workspace_bytes < part_bytes(p, heads) || (part_bytes(p, heads) > 0 && !workspace))
+    const int terms = dtype == MXQ_DTYPE_F16 ? 2 : 1;
+    const Plan p = make_plan(requests, rows, q_heads / heads, max_new, width * page_size, heads, a.c.nb, terms);
+    const int64_t needed = part_bytes(p, heads, terms, requests);
+    // units and items are numbered in 32 bits
+    const int64_t most_units = (requests + ceil_div(rows * q_heads / heads, 16)) * (ceil_div(width * page_size, KV_UNIT) + 1);
+    // .. and so are the workgroups of a launch
+    if (most_units > 0x7FFFFFFF || p.prompt_items * heads * 16 + (int64_t)64 * requests * heads > 0x7FFFFFFF || p.decode_items * heads > 0x7FFFFFFF) return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
+    if (workspace_bytes < needed || (needed > 0 && !workspace))
         return fail(MXQ_ERR_ARGUMENT, "%s: the workspace is too small", who);
-    if (reinterpret_cast<uintptr_t>(workspace) & 7) return fail(MXQ_ERR_ARGUMENT, "%s: the workspace must be 8-byte aligned", who);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(MXQ_ERR_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
     a.q = reinterpret_cast<const unsigned short*>(q);
     a.q_token = q_token_stride;
     a.q_head = q_head_stride;
@@ -227,7 +248,8 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.group = q_heads / heads;
     a.rows = rows;
     a.scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
-    a.q_sign = scale < 0 ? 0x80008000u : 0u;
+    if (a.scale_log2 < 1.17549435e-38f) a.scale_log2 = 1.17549435e-38f;      // 0 times a masked score of -inf would be NaN
+    a.negative = scale < 0 ? 1 : 0;
     a.causal = causal ? 1 : 0;
     a.q_wide = aligned16(q) && head_dim % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     a.out_wide = aligned16(out) && head_dim % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0;
@@ -235,17 +257,27 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.tile_columns = 16 * p.ct;
     a.decode_columns = p.decode_columns;
     a.whole = p.whole ? 1 : 0;
+    a.direct = p.whole && !starts && a.group <= 16 * p.ct ? 1 : 0;
     a.shares = (int)p.shares;
+    a.join_rows = p.prompt ? p.decode_columns / a.group : 0;
     a.part = reinterpret_cast<float*>(workspace);
+    unsigned char* behind = reinterpret_cast<unsigned char*>(workspace) + decode_part_bytes(p, heads);
+    a.prompt_part = p.prompt ? reinterpret_cast<float*>(behind) : nullptr;
+    a.plan = p.prompt ? behind + prompt_part_bytes(p, heads, terms) : nullptr;
+    a.prompt_shares = (int)p.prompt_shares;
+    a.prompt_items = (int)p.prompt_items;
+    // requests with few columns have few rows where the others are the prompt kernel's
+    const int64_t join = p.whole ? 0 : (p.prompt ? a.join_rows * requests : rows) * q_heads;
+    a.join_blocks = (int)join;
     hipStream_t s = (hipStream_t)hip_stream;
     mxq_kv::launch_decode(dtype, &a, p, s);
-    rc = check_launch(who);
-    if (rc) return rc;
+    if ((rc = check_launch(who))) return rc;
     if (p.prompt) {
         mxq_kv::launch_prompt(dtype, &a, p, s);
-        rc = check_launch(who);
+        if ((rc = check_launch(who))) return rc;
     }
-    return rc;
+    mxq_kv::launch_join(dtype, &a, p, s);
+    return check_launch(who);
 }
 
 }  // extern "C"

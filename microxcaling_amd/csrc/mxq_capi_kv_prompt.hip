@@ -1,12 +1,12 @@
-// Launches of the prompt kernel of the packed cache's attention.
+// Launch of the prompt kernel of the packed cache's attention.
 #include "mxq_capi_kv.h"
 
 namespace {
 
 template <int DT>
 void launch(const KvAttnArgs& a, const mxq_kv::Plan& p, hipStream_t s) {
-    const unsigned grid = (unsigned)(p.prompt_tiles * a.c.heads);
-    MXQ_KV_CASES(p.nb, constexpr int CT = kv_prompt_ct(NB); kv_prompt_kernel<DT, NB, CT><<<grid, kThreads, 0, s>>>(a))
+    const unsigned grid = (unsigned)(p.prompt_shares * a.c.heads);
+    MXQ_KV_CASES(p.nb, constexpr int CT = kv_prompt_ct(NB, kv_terms<DT>()); kv_prompt_kernel<DT, NB, CT><<<grid, kThreads, 0, s>>>(a))
 }
 
 }  // namespace

@@ -24,6 +24,7 @@
 
 namespace {
 
+typedef float kv_f32x2 __attribute__((ext_vector_type(2)));
 typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 kv_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 kv_bf16x2 __attribute__((ext_vector_type(2)));
@@ -36,7 +37,12 @@ struct KvCache {
     int64_t num_pages;
     int64_t record;                                      // bytes of a (page, head)
     int heads, page_size, head_dim, nb;
+    uint32_t divide_by, shift_by;                        // n / page_size = (h + (n - h >> 1)) >> shift_by, h = high half of n divide_by
 };
+__device__ __forceinline__ uint32_t kv_page_of(const KvCache& c, uint32_t n) {
+    const uint32_t h = (uint32_t)(((uint64_t)n * c.divide_by) >> 32);
+    return (h + ((n - h) >> 1)) >> c.shift_by;
+}
 
 // ---- exchanges between the four lane groups of 16 -------------------------------------------------------------
 // f(v of this lane, v of lane ^ 16), then the same with lane ^ 32: a reduction over the groups, in every lane
@@ -60,33 +66,47 @@ __device__ __forceinline__ uint32_t or_over_groups(uint32_t v) {
     return b[0] | b[1];
 }
 __device__ __forceinline__ bool any_lane(bool p) { return !__all(!p); }
+// a value that is the same in every lane of the wave, told to the compiler: it goes to a scalar register, and branches
+// and addresses that follow from it stay scalar too
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+    const uint32_t lo = (uint32_t)uniform((int)(uint32_t)v), hi = (uint32_t)uniform((int)(uint32_t)((uint64_t)v >> 32));
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
 
-// sum over the workgroup, in every thread (s: one int64 for each wave)
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* s) {
+template <class T>
+__device__ __forceinline__ T uniform_any(T v) {
+    if constexpr (sizeof(T) == 8) return uniform64(v);
+    else return uniform(v);
+}
+// sum over the workgroup, in every thread (s: a value for each wave)
+template <class T>
+__device__ __forceinline__ T block_sum(T v, T* s) {
     for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
     for (int w = 0; w < TPB / 64; ++w) v += s[w];
-    return v;
+    return uniform_any(v);
 }
 // inclusive prefix sum over the workgroup's threads; *total: their sum
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s, int64_t* total) {
+template <class T>
+__device__ __forceinline__ T block_scan(T v, T* s, T* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up(v, d, 64);
+        const T o = __shfl_up(v, d, 64);
         if (lane >= d) v += o;
     }
     __syncthreads();
     if (lane == 63) s[wave] = v;
     __syncthreads();
-    int64_t t = 0;
+    T t = 0;
     for (int w = 0; w < TPB / 64; ++w) {
         if (w == wave) v += t;
         t += s[w];
     }
-    *total = t;
+    *total = uniform_any(t);
     return v;
 }
 

@@ -34,19 +34,25 @@ struct KvAttnArgs {
     int requests, group;                                 // query heads of a kv head
     int64_t rows;                                        // rows of q and out
     float scale_log2;                                    // |scale| log2(e)
-    unsigned q_sign;                                     // 0x80008000 where scale is negative
+    int negative;                                        // scale is
     int causal, q_wide, out_wide, zero_tail;
     int tile_columns;                                    // decode: columns of an item, 16 CT
     int decode_columns;                                  // requests with more columns belong to the prompt kernel
     int whole;                                           // decode: a workgroup for each item, nothing to join
-    int shares;                                          // decode: workgroups of a kv head
+    int direct;                                          // .. and one item for each request
+    int shares;                                          // decode: workgroups of a kv head, at most KV_MAX_SHARES
+    int join_rows;                                       // join: so many rows of each request, or 0: every row
     float* part;                                         // decode: partial results, two places for each workgroup
+    int join_blocks;                                     // join: workgroups for decode rows, the others for prompt items
+    int prompt_shares, prompt_items;                     // prompt: workgroups of a kv head and items of it, at most
+    float* prompt_part;
+    void* plan;                                          // null: no prompt kernel
     KvCache c;
 };
 
 // a request as the attention sees it
 struct KvSeq {
-    int64_t row0;                                        // its first row of q
+    int row0;                                            // its first row of q
     int fresh;                                           // its rows
     int len;                                             // tokens, unlimited
     int keys;                                            // tokens that the table can name
@@ -54,18 +60,19 @@ struct KvSeq {
 __device__ __forceinline__ KvSeq kv_seq(const KvAttnArgs& a, int r) {
     KvSeq s;
     if (a.starts) {
-        int64_t s0 = a.starts[r], s1 = a.starts[r + 1];
-        s0 = s0 < 0 ? 0 : (s0 < a.rows ? s0 : a.rows);
-        s1 = s1 < s0 ? s0 : (s1 < a.rows ? s1 : a.rows);
+        const int rows = (int)a.rows;                    // (below 2^31)
+        int s0 = a.starts[r], s1 = a.starts[r + 1];
+        s0 = s0 < 0 ? 0 : (s0 < rows ? s0 : rows);
+        s1 = s1 < s0 ? s0 : (s1 < rows ? s1 : rows);
         s.row0 = s0;
-        s.fresh = (int)(s1 - s0);
+        s.fresh = s1 - s0;
     } else {
         s.row0 = r;
         s.fresh = 1;
     }
     s.len = a.seq_lens[r] > 0 ? a.seq_lens[r] : 0;
-    const int64_t room = (int64_t)a.width * a.c.page_size;
-    s.keys = s.len < room ? s.len : (int)room;
+    const int room = a.width * a.c.page_size;            // (at most 2^30)
+    s.keys = s.len < room ? s.len : room;
     return s;
 }
 // keys that new token i sees (0 or less: none)
@@ -75,41 +82,51 @@ __device__ __forceinline__ int kv_limit(const KvAttnArgs& a, const KvSeq& s, int
     return n < s.keys ? (int)(n > 0 ? n : 0) : s.keys;
 }
 
+// the running maximum before anything has been seen: below every score, but finite, so that neither a difference of two
+// of them nor one with a masked score's -inf is NaN
+constexpr float KV_NOTHING = -3.0e38f;
+constexpr int KV_MAX_SHARES = 1024;
 constexpr int KV_UNIT = 128;                             // tokens of a unit of work: a tile of 32 for each wave
 
 // units and column groups of a request in the decode kernel; a request without keys still has one unit, whose
 // workgroup writes the zeros
 struct KvWork {
     int units, groups;
+    __device__ __forceinline__ int count() const { return units * groups; }  // (all of them together: below 2^31)
 };
 __device__ __forceinline__ KvWork kv_work(const KvAttnArgs& a, const KvSeq& s) {
-    const int64_t columns = (int64_t)s.fresh * a.group;
+    const int columns = s.fresh * a.group;
     if (columns == 0 || columns > a.decode_columns) return KvWork{0, 0};
     const int units = (s.keys + KV_UNIT - 1) / KV_UNIT;
-    return KvWork{units > 0 ? units : 1, (int)((columns + a.tile_columns - 1) / a.tile_columns)};
+    return KvWork{units > 0 ? units : 1, (columns + a.tile_columns - 1) / a.tile_columns};
 }
 
 // ---- loads -------------------------------------------------------------------------------------------------------
+// Memory that is named by a uniform address, a uniform distance from it and an offset of the lane's own: buffer loads take
+// the three as they are, without arithmetic in vector registers.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv_buffer(const unsigned char* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(base), 0, 0xFFFFFFFF, 0x00027000);
+}
 // N dwords from an address that is aligned to min(4 N, 16) bytes where N is a power of two, to 4 otherwise
 template <int N>
-__device__ __forceinline__ void load_dwords(const unsigned char* p, uint32_t* d) {
+__device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t from, int lane_offset, int offset, uint32_t* d) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
-            const u32x4 w = reinterpret_cast<const u32x4*>(p)[i];
+            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset + 16 * i, offset, 0));
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[4 * i + e] = w[e];
         }
     } else if constexpr (N % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-            const u32x2 w = reinterpret_cast<const u32x2*>(p)[i];
+            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(from, lane_offset + 8 * i, offset, 0));
             d[2 * i] = w[0];
             d[2 * i + 1] = w[1];
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) d[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        for (int i = 0; i < N; ++i) d[i] = __builtin_amdgcn_raw_buffer_load_b32(from, lane_offset + 4 * i, offset, 0);
     }
 }
 
@@ -122,19 +139,18 @@ __device__ __forceinline__ uint32_t kv_k_scale(const uint32_t* ks, int g, int s)
     constexpr int N = kv_k_scales<NB>();
     if constexpr (N == 1) return ks[0];
     if constexpr (NB % 4 == 0) return ks[s / 4];
-    const int at = (NB * g + s) / 4 - NB * g / 4;
-    uint32_t v = ks[0];
+    uint32_t all = ks[0];                                // bytes side by side, picked by a shift
 #pragma unroll
-    for (int k = 1; k < N; ++k) v = at == k ? ks[k] : v;
-    return v;
+    for (int k = 1; k < N; ++k) all |= ks[k] << (8 * k);
+    return all >> (8 * ((NB * g + s) / 4 - NB * g / 4));  // what is above the byte is shifted out or ignored
 }
 
-template <int NB>
-struct KvTile {                                          // what a lane holds of 32 tokens
-    uint32_t k[2][NB], ks[2][kv_k_scales<NB>()];
-    uint32_t v[2][NB], vs[2][NB];
-    bool there[2];                                       // the two pages exist (uniform over the wave)
-};
+// A copy of a value that the compiler takes for a new one.  What rarely taken branches work out from a lane's number would
+// otherwise be worked out before the loops around them and occupy registers throughout (16 of them for the masks).
+__device__ __forceinline__ int here_only(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // the scale operand of v_cvt_scalef32_*: only the exponent field counts (255: NaN, 0: 2^-127)
 template <int SEL>
@@ -148,52 +164,120 @@ template <int SEL>                                       // exponent field of by
 __device__ __forceinline__ uint32_t kv_scale_bits(uint32_t four) {
     return SEL == 3 ? four >> 1 : four << (23 - 8 * SEL);
 }
+// eight K elements of a lane as an operand
+__device__ __forceinline__ kv_bf16x8 kv_k_operand(uint32_t codes, uint32_t scale) {
+    const uint32_t bits = scale << 23;
+    return kv_operand(kv_decode2<0>(codes, bits), kv_decode2<1>(codes, bits), kv_decode2<2>(codes, bits),
+                      kv_decode2<3>(codes, bits));
+}
+// the two V operands of a block from a lane's codes and scales of two groups of four tokens
+__device__ __forceinline__ void kv_v_operands(const uint32_t codes[2], const uint32_t scales[2], kv_bf16x8 out[2]) {
+    uint32_t cv[8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        cv[4 * j + 0] = kv_decode2<0>(codes[j], kv_scale_bits<0>(scales[j]));
+        cv[4 * j + 1] = kv_decode2<1>(codes[j], kv_scale_bits<1>(scales[j]));
+        cv[4 * j + 2] = kv_decode2<2>(codes[j], kv_scale_bits<2>(scales[j]));
+        cv[4 * j + 3] = kv_decode2<3>(codes[j], kv_scale_bits<3>(scales[j]));
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const uint32_t sel = n ? 0x07060302u : 0x05040100u;                  // the upper or lower halves of two dwords
+        out[n] = kv_operand(__builtin_amdgcn_perm(cv[1], cv[0], sel), __builtin_amdgcn_perm(cv[3], cv[2], sel),
+                            __builtin_amdgcn_perm(cv[5], cv[4], sel), __builtin_amdgcn_perm(cv[7], cv[6], sel));
+    }
+}
 
+// The V scales of a masked tile of 32 tokens (t0 ..; a lane: tokens 4 g + r of halves j): tokens behind `end` or on
+// missing pages and tokens whose block is NaN get the scale 2^-127, since even a probability of 0 times NaN is NaN.
+// Returns which of the 32 tokens have a NaN block; their columns are told by kv_spread_nan.
+__device__ __forceinline__ uint32_t kv_mend_scales(uint32_t scales[2], const bool there[2], int t0, int g, int end) {
+    uint32_t nan = 0;
+    g = here_only(g);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool seen = there[j] && t0 + 16 * j + 4 * g + r < end;
+            const bool is_nan = ((scales[j] >> (8 * r)) & 255u) == 255u;
+            if (is_nan && seen) nan |= 1u << (16 * j + 4 * g + r);
+            if (is_nan || !seen) scales[j] &= ~(255u << (8 * r));
+        }
+    return nan;
+}
+
+// Eight 16-bit elements e0 .. of a row that ends at `end`, where rows are not aligned.  A loop, not unrolled: unrolled,
+// its conditions would occupy scalar registers through the kernels' main loops.
+__device__ __forceinline__ void kv_store8_unaligned(unsigned short* row, int e0, int end, u32x4 w) {
+    const uint64_t half[2] = {(uint64_t)w[1] << 32 | w[0], (uint64_t)w[3] << 32 | w[2]};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma nounroll
+        for (int e = 0; e < 4; ++e)
+            if (e0 + 4 * h + e < end) row[e0 + 4 * h + e] = (unsigned short)(half[h] >> (16 * e));
+}
+
+template <int NB>
+struct KvKeys {                                          // what a lane holds of 32 tokens' keys ..
+    uint32_t k[2][NB], ks[2][kv_k_scales<NB>()];
+};
+template <int NB>
+struct KvValues {                                        // .. and values
+    uint32_t v[2][NB], vs[2][NB];
+};
+
+// the columns of a wave
 template <int NB, int CT, int NT, int NP>
 struct KvWave {
     kv_f32x4 acc[CT][NB][2];                             // element 32 b + 2 (4 g + r) + n of the lane's column
     float m[CT], l[CT];                                  // l: this lane's tokens only
     kv_bf16x8 q[CT][NT][NB];
-    int limit[CT];                                       // keys that the lane's column sees
+    uint32_t limits;                                     // keys that the lane's columns see beyond min_limit: 8 bits each
+    bool started;                                        // every column has seen a token (uniform)
     int min_limit, max_limit;                            // over the wave's columns
-    const unsigned char* base;                           // of the kv head
     int lane, i16, g;
 
-    // columns c0 .. c0 + 16 CT - 1 of request s
-    __device__ __forceinline__ void begin(const KvAttnArgs& a, const KvSeq& s, int head, int c0) {
+    // Columns c0 .. c0 + 16 CT - 1 of request s.  Called by all waves of the workgroup; stage: 32 NB x 16 16-bit elements
+    // of LDS for each wave, which q passes through where its rows are not aligned.
+    __device__ __forceinline__ void begin(const KvAttnArgs& a, const KvSeq& s, int head, int c0, unsigned short* stage) {
         lane = threadIdx.x & 63;
         i16 = lane & 15;
         g = lane >> 4;
-        base = a.c.data + (int64_t)head * a.c.record;
         const int columns = s.fresh * a.group;
         const int last = (c0 + 16 * CT < columns ? c0 + 16 * CT : columns) - 1;
         min_limit = kv_limit(a, s, c0 / a.group);
         max_limit = kv_limit(a, s, last / a.group);
+        started = false;
+        limits = 0;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            m[ct] = -__builtin_inff();
+            m[ct] = KV_NOTHING;
             l[ct] = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[ct][b][0] = acc[ct][b][1] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             const int c = c0 + 16 * ct + i16, token = c / a.group;
             const bool live = c < columns;
-            limit[ct] = live ? kv_limit(a, s, token) : max_limit;
-            const unsigned short* row = a.q + (s.row0 + (live ? token : 0)) * a.q_token +
+            limits |= (uint32_t)((live ? kv_limit(a, s, token) : max_limit) - min_limit) << (8 * ct);   // (at most 16 CT tokens apart)
+            const unsigned short* row = a.q + (int64_t)(s.row0 + (live ? token : 0)) * a.q_token +
                                         ((int64_t)head * a.group + (live ? c - token * a.group : 0)) * a.q_head;
+            if (!a.q_wide) {
+                __syncthreads();                         // what was there has been read
+#pragma nounroll
+                for (int e = here_only(lane); e < 16 * 32 * NB; e += 64) {
+                    const int x = c0 + 16 * ct + e / (32 * NB), d = e % (32 * NB), t = x / a.group;
+                    unsigned short v = 0;
+                    if (x < columns && d < a.c.head_dim)
+                        v = a.q[(int64_t)(s.row0 + t) * a.q_token + ((int64_t)head * a.group + (x - t * a.group)) * a.q_head + d];
+                    stage[e] = v;
+                }
+                __syncthreads();
+            }
 #pragma unroll
             for (int st = 0; st < NB; ++st) {
                 const int e0 = 8 * NB * g + 8 * st;
                 u32x4 w = {0, 0, 0, 0};
-                if (live && e0 < a.c.head_dim) {
-                    if (a.q_wide) {
-                        w = *reinterpret_cast<const u32x4*>(row + e0);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (e0 + e < a.c.head_dim) w[e / 2] |= (uint32_t)row[e0 + e] << (16 * (e & 1));
-                    }
-                    w ^= a.q_sign;
-                }
+                if (!a.q_wide) w = *reinterpret_cast<const u32x4*>(stage + i16 * (32 * NB) + e0);
+                else if (live && e0 < a.c.head_dim) w = *reinterpret_cast<const u32x4*>(row + e0);
                 if constexpr (NT == 1) {
                     q[ct][0][st] = __builtin_bit_cast(kv_bf16x8, w);
                 } else {                                 // fp16: 11 bits as 8 + the rest, both exact
@@ -213,91 +297,73 @@ struct KvWave {
         }
     }
 
-    // tokens 16 sub .. of page `page` (negative: none), as sub-tile j
-    __device__ __forceinline__ void load_half(const KvAttnArgs& a, KvTile<NB>& t, int j, int page, int sub) const {
-        t.there[j] = page >= 0;
-        const int ps = a.c.page_size;
-        const unsigned char* rec = base + (int64_t)(page >= 0 ? page : 0) * ((int64_t)a.c.heads * a.c.record);
-        const int off = 16 * (page >= 0 ? sub : 0);
-        load_dwords<NB>(rec + (off + i16) * (16 * NB) + g * (4 * NB), t.k[j]);
-        const unsigned char* vt = rec + ps * (16 * NB) + (off / 4 + g) * (64 * NB);
-        load_dwords<NB>(vt + i16 * (4 * NB), t.v[j]);
-        const unsigned char* ks = rec + ps * (32 * NB) + (off + i16) * NB;
+    __device__ __forceinline__ int limit(int ct) const { return min_limit + (int)(limits >> (8 * ct) & 255u); }
+
+    // sc (+)= (operand of half j, step st) x q
+    __device__ __forceinline__ void multiply_keys(const kv_bf16x8& k8, int j, int st, kv_f32x4 sc[CT][2]) const {
 #pragma unroll
-        for (int k = 0; k < kv_k_scales<NB>(); ++k) {
-            const int b = NB * g / 4 + k;
-            t.ks[j][k] = ks[b < NB ? b : NB - 1];
-        }
-        load_dwords<NB>(rec + ps * (33 * NB) + (off / 4 + g) * (4 * NB), t.vs[j]);
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                sc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    k8, q[ct][nt][st], st == 0 && nt == 0 ? kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f} : sc[ct][j], 0, 0, 0);
     }
 
-    // tokens t0 .. t0 + 31
-    __device__ __forceinline__ void step(const KvAttnArgs& a, KvTile<NB>& t, int t0) {
-        kv_f32x4 sc[CT][2];
+    // scores of 32 tokens from t0 to probabilities, in place of which the maximum and the sums follow
+    __device__ __forceinline__ void probabilities(const KvAttnArgs& a, kv_f32x4 sc[CT][2], bool masked, const bool there[2], int t0,
+                                                  uint32_t p_hi[CT][4], uint32_t p_lo[CT][4]) {
+        if (a.negative) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) sc[ct][0] = sc[ct][1] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int st = 0; st < NB; ++st) {
-                const uint32_t bits = kv_k_scale<NB>(t.ks[j], g, st) << 23, w = t.k[j][st];
-                const kv_bf16x8 k8 = kv_operand(kv_decode2<0>(w, bits), kv_decode2<1>(w, bits), kv_decode2<2>(w, bits),
-                                                kv_decode2<3>(w, bits));
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        sc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, q[ct][nt][st], sc[ct][j], 0, 0, 0);
+            for (int ct = 0; ct < CT; ++ct) {
+                sc[ct][0] = -sc[ct][0];
+                sc[ct][1] = -sc[ct][1];
             }
-        // a tile that every column sees entirely needs no mask
-        const bool masked = t0 + 32 > min_limit || !t.there[0] || !t.there[1];
-        uint32_t nan_of[NB];                             // masked tiles: which of the 32 tokens have a NaN block b of V
-        bool any_nan = false;
-        if (masked) {
-            uint32_t mine = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) nan_of[b] = 0;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int token = t0 + 16 * j + 4 * g + r;
-                    const bool seen = t.there[j] && token < max_limit;
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const uint32_t byte = (t.vs[j][b] >> (8 * r)) & 255u;
-                        const bool nan = byte == 255u;
-                        if (nan && seen) nan_of[b] |= 1u << (16 * j + 4 * g + r);
-                        if (nan || !seen) t.vs[j][b] &= ~(255u << (8 * r));     // 0 x NaN must not reach a column that
-                    }                                                           // does not see the token
-                }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) mine |= nan_of[b];
-            any_nan = any_lane(mine != 0u);
         }
-        uint32_t p_hi[CT][4], p_lo[CT][NP == 2 ? 4 : 1];
+        if (masked) {
+            const int first = t0 + 4 * here_only(g);
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            float p[8];
-            if (masked) {
+            for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const bool seen = t.there[e >> 2] && t0 + 16 * (e >> 2) + 4 * g + (e & 3) < limit[ct];
-                    p[e] = seen ? sc[ct][e >> 2][e & 3] * a.scale_log2 : -__builtin_inff();
+                    const bool seen = there[e >> 2] && first + 16 * (e >> 2) + (e & 3) < limit(ct);
+                    sc[ct][e >> 2][e & 3] = seen ? sc[ct][e >> 2][e & 3] : -__builtin_inff();
                 }
-            } else {
+        }
+        if (!started) {                                  // columns that have not seen a token yet begin with this tile's maximum
+            bool waiting = false;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = sc[ct][e >> 2][e & 3] * a.scale_log2;
+            for (int ct = 0; ct < CT; ++ct) {
+                float mx = sc[ct][0][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) mx = __builtin_fmaxf(mx, sc[ct][e >> 2][e & 3]);
+                mx = max_over_groups(mx) * a.scale_log2; // (a scale of 0 is passed as the smallest normal number)
+                if (m[ct] == KV_NOTHING) m[ct] = mx > KV_NOTHING ? mx : KV_NOTHING;
+                waiting |= m[ct] == KV_NOTHING;
             }
-            float mx = p[0];
+            started = !any_lane(waiting);
+        }
+        // s - m; m is raised, and only then do the lane groups compare, after a jump by more than 8
+        bool jump = false;
+        float over[CT];
 #pragma unroll
-            for (int e = 1; e < 8; ++e) mx = __builtin_fmaxf(mx, p[e]);
-            mx = max_over_groups(mx);
-            if (any_lane(mx > m[ct] + 8.0f)) {           // -inf at first
-                const float up = mx > m[ct] + 8.0f ? mx : m[ct];
-                const float f = up > m[ct] ? __builtin_amdgcn_exp2f(m[ct] - up) : 1.0f;
-                m[ct] = up;
+        for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                sc[ct][e >> 2][e & 3] = __builtin_fmaf(sc[ct][e >> 2][e & 3], a.scale_log2, -m[ct]);
+            over[ct] = sc[ct][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) over[ct] = __builtin_fmaxf(over[ct], sc[ct][e >> 2][e & 3]);
+            jump |= over[ct] > 8.0f;
+        }
+        if (any_lane(jump)) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const float top = max_over_groups(over[ct]), up = top > 8.0f ? top : 0.0f;
+                const float f = __builtin_amdgcn_exp2f(-up);                 // 1 where m stays
+                m[ct] += up;
                 l[ct] *= f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sc[ct][e >> 2][e & 3] -= up;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -305,9 +371,12 @@ struct KvWave {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[ct][b][n][r] *= f;
             }
-            const float mm = m[ct] == -__builtin_inff() ? 0.0f : m[ct];      // nothing seen yet: 2^-inf = 0
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(p[e] - mm);
+        for (int ct = 0; ct < CT; ++ct) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(sc[ct][e >> 2][e & 3]);
             l[ct] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
@@ -317,94 +386,182 @@ struct KvWave {
                                                       p[2 * d + 1] - Pack<MXQ_BF16>::get(p_hi[ct][d], 1));
             }
         }
+    }
+
+    // acc += (V operand n of block b) x probabilities
+    __device__ __forceinline__ void multiply_values(const kv_bf16x8& v8, int b, int n, const uint32_t p_hi[CT][4],
+                                                    const uint32_t p_lo[CT][4]) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            uint32_t cv[8];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                cv[4 * j + 0] = kv_decode2<0>(t.v[j][b], kv_scale_bits<0>(t.vs[j][b]));
-                cv[4 * j + 1] = kv_decode2<1>(t.v[j][b], kv_scale_bits<1>(t.vs[j][b]));
-                cv[4 * j + 2] = kv_decode2<2>(t.v[j][b], kv_scale_bits<2>(t.vs[j][b]));
-                cv[4 * j + 3] = kv_decode2<3>(t.v[j][b], kv_scale_bits<3>(t.vs[j][b]));
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const uint32_t sel = n ? 0x07060302u : 0x05040100u;          // the upper or lower halves of two dwords
-                const kv_bf16x8 v8 = kv_operand(
-                    __builtin_amdgcn_perm(cv[1], cv[0], sel), __builtin_amdgcn_perm(cv[3], cv[2], sel),
-                    __builtin_amdgcn_perm(cv[5], cv[4], sel), __builtin_amdgcn_perm(cv[7], cv[6], sel));
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    acc[ct][b][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        v8, kv_operand(p_hi[ct][0], p_hi[ct][1], p_hi[ct][2], p_hi[ct][3]), acc[ct][b][n], 0, 0, 0);
-                    if constexpr (NP == 2)
-                        acc[ct][b][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            v8, kv_operand(p_lo[ct][0], p_lo[ct][1], p_lo[ct][2], p_lo[ct][3]), acc[ct][b][n], 0, 0, 0);
-                }
-            }
+        for (int ct = 0; ct < CT; ++ct) {
+            acc[ct][b][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                v8, kv_operand(p_hi[ct][0], p_hi[ct][1], p_hi[ct][2], p_hi[ct][3]), acc[ct][b][n], 0, 0, 0);
+            if constexpr (NP == 2)
+                acc[ct][b][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    v8, kv_operand(p_lo[ct][0], p_lo[ct][1], p_lo[ct][2], p_lo[ct][3]), acc[ct][b][n], 0, 0, 0);
         }
-        if (any_nan) {                                   // rare: the NaN blocks reach the columns that see them
+    }
+
+    // block b is NaN in the tokens `of` (of 32 from t0): so is it in the columns that see one of them
+    __device__ __forceinline__ void spread_nan(int b, uint32_t of, int t0) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint32_t of = or_over_groups(nan_of[b]);
+        for (int ct = 0; ct < CT; ++ct) {
+            const int n = limit(ct) - t0;
+            const uint32_t sees = n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u;
+            if (of & sees) {
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    const int n = limit[ct] - t0;
-                    const uint32_t sees = n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u;
-                    if (of & sees) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[ct][b][0][r] = acc[ct][b][1][r] = mxq_float(MXQ_QNAN_BITS);
-                    }
-                }
+                for (int r = 0; r < 4; ++r) acc[ct][b][0][r] = acc[ct][b][1][r] = mxq_float(MXQ_QNAN_BITS);
             }
         }
     }
 
-    // the tiles first, first + stride, .. of 32 tokens below tile `end`: the pages of 32 tiles at a time sit in the
-    // lanes (lane: tile lane / 2, half lane % 2), and a tile's codes are on their way while the one before is multiplied
-    __device__ __forceinline__ void walk(const KvAttnArgs& a, int r, int first, int end, int stride) {
-        const int subs = a.c.page_size / 16;
+    // ---- straight from memory (the decode kernel) ----
+    // a lane's constant offsets into the halves of a tile
+    int at_k, at_v, at_ks[kv_k_scales<NB>()], at_vs;
+    __device__ __forceinline__ void place(const KvAttnArgs& a) {
+        const int ps = a.c.page_size;
+        at_k = i16 * (16 * NB) + g * (4 * NB);
+        at_v = ps * (16 * NB) + g * (64 * NB) + i16 * (4 * NB);
+        at_vs = ps * NB + g * (4 * NB);
+#pragma unroll
+        for (int k = 0; k < kv_k_scales<NB>(); ++k) {
+            const int b = NB * g / 4 + k;
+            at_ks[k] = i16 * NB + (b < NB ? b : NB - 1);
+        }
+    }
+    // 16 tokens in the cache, for the loads of a wave: where their K codes lie (V's are a page's K codes further), how far
+    // it is from there to their K scales (V's are a page's K scales further), and whether the page exists (else: the
+    // first tokens of the cache, whose scores are masked)
+    struct Spot {
+        int64_t codes;
+        int scales;
+        bool there;
+    };
+    __device__ __forceinline__ static Spot spot(const KvAttnArgs& a, const int* row, int head, int sub, int end) {
+        const int subs = a.c.page_size / 16, at = sub / subs;
+        int page = -1, in_page = 0;
+        if (at < a.width && sub < end) {
+            page = row[at];
+            if (page >= a.c.num_pages) page = -1;
+            if (page >= 0) in_page = sub - at * subs;
+        }
+        Spot p;
+        p.there = page >= 0;
+        p.codes = ((int64_t)(page >= 0 ? page : 0) * a.c.heads + head) * a.c.record + in_page * (256 * NB);
+        p.scales = a.c.page_size * (32 * NB) - in_page * (240 * NB);
+        return p;
+    }
+    __device__ __forceinline__ static __amdgpu_buffer_rsrc_t lane_codes(const KvAttnArgs& a, const Spot& p, int l) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)p.codes, l);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)p.codes >> 32), l);
+        return kv_buffer(a.c.data + (((uint64_t)hi << 32) | lo));
+    }
+    __device__ __forceinline__ void fetch_keys(const KvAttnArgs& a, KvKeys<NB>& t, const Spot& p, int n) const {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const __amdgpu_buffer_rsrc_t from = lane_codes(a, p, 2 * n + j);
+            const int scales = __builtin_amdgcn_readlane(p.scales, 2 * n + j);
+            load_dwords<NB>(from, at_k, 0, t.k[j]);
+#pragma unroll
+            for (int k = 0; k < kv_k_scales<NB>(); ++k) t.ks[j][k] = __builtin_amdgcn_raw_buffer_load_b8(from, at_ks[k], scales, 0);
+        }
+    }
+    __device__ __forceinline__ void fetch_values(const KvAttnArgs& a, KvValues<NB>& t, const Spot& p, int n) const {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const __amdgpu_buffer_rsrc_t from = lane_codes(a, p, 2 * n + j);
+            load_dwords<NB>(from, at_v, 0, t.v[j]);
+            load_dwords<NB>(from, at_vs, __builtin_amdgcn_readlane(p.scales, 2 * n + j), t.vs[j]);
+        }
+    }
+
+    // The tiles first, first + stride, .. of 32 tokens below tile `end`.  The places of 32 tiles sit in the lanes (lane:
+    // tile lane / 2, half lane % 2).  DEPTH tiles are under way: a tile's keys are loaded as soon as those that lay in
+    // the same registers have been multiplied, its values likewise.
+    template <int DEPTH>
+    __device__ __forceinline__ void walk(const KvAttnArgs& a, int r, int head, int first, int end, int stride) {
         const int seen_end = (max_limit + 31) / 32;      // uniform: nothing behind it is seen
         if (end > seen_end) end = seen_end;
+        place(a);
         const int* row = a.table + (int64_t)r * a.table_stride;
         for (int chunk = first; chunk < end; chunk += 32 * stride) {
-            const int sub = 2 * (chunk + (lane >> 1) * stride) + (lane & 1);
-            int page = -1, in_page = 0;
-            const int at = sub / subs;
-            if (at < a.width && sub * 16 < max_limit) {
-                page = row[at];
-                in_page = sub - at * subs;
-                if (page >= a.c.num_pages) page = -1;
-            }
-            KvTile<NB> next;
-            load_half(a, next, 0, __builtin_amdgcn_readlane(page, 0), __builtin_amdgcn_readlane(in_page, 0));
-            load_half(a, next, 1, __builtin_amdgcn_readlane(page, 1), __builtin_amdgcn_readlane(in_page, 1));
+            const Spot p = spot(a, row, head, 2 * (chunk + (lane >> 1) * stride) + (lane & 1), (max_limit + 15) / 16);
+            const uint64_t there = __ballot(p.there);
             int tiles = (end - chunk + stride - 1) / stride;
             if (tiles > 32) tiles = 32;
-            for (int n = 0; n < tiles; ++n) {
-                KvTile<NB> now = next;
-                if (n + 1 < tiles) {
-                    load_half(a, next, 0, __builtin_amdgcn_readlane(page, 2 * n + 2), __builtin_amdgcn_readlane(in_page, 2 * n + 2));
-                    load_half(a, next, 1, __builtin_amdgcn_readlane(page, 2 * n + 3), __builtin_amdgcn_readlane(in_page, 2 * n + 3));
-                }
-                step(a, now, 32 * (chunk + n * stride));
+            KvKeys<NB> keys[DEPTH];
+            KvValues<NB> values[DEPTH];
+            // no load is conditional: behind the last tile it is loaded again, and multiplied with nothing of it seen.
+            // The waits count the loads under way, and a branch around one would make them wait for more than needed.
+            const int last = tiles - 1;
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                // in the order of the loop's loads, on which its waits rely
+                fetch_keys(a, keys[d], p, d < last ? d : last);
+                __builtin_amdgcn_sched_barrier(0);
+                fetch_values(a, values[d], p, d < last ? d : last);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            for (int n0 = 0; n0 < tiles; n0 += DEPTH) {
+#pragma unroll
+                for (int d = 0; d < DEPTH; ++d) {
+                    const int n = n0 + d, after = n + DEPTH < last ? n + DEPTH : last;
+                    step(a, keys[d], values[d], p, n <= last ? (int)(there >> (2 * n)) & 3 : 0, after, 32 * (chunk + n * stride));
+                }
+            }
+        }
+    }
+    // the tokens t0 .. (there_bits: which halves exist) from their registers, which then take tile `after`
+    __device__ __forceinline__ void step(const KvAttnArgs& a, KvKeys<NB>& keys, KvValues<NB>& values, const Spot& p, int there_bits,
+                                         int after, int t0) {
+        kv_f32x4 sc[CT][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int st = 0; st < NB; ++st)
+                multiply_keys(kv_k_operand(keys.k[j][st], kv_k_scale<NB>(keys.ks[j], g, st)), j, st, sc);
+        fetch_keys(a, keys, p, after);
+        // a tile that every column sees entirely needs no mask
+        const bool there[2] = {(there_bits & 1) != 0, (there_bits & 2) != 0};
+        const bool masked = t0 + 32 > min_limit || there_bits != 3;
+        uint32_t p_hi[CT][4], p_lo[CT][4];
+        probabilities(a, sc, masked, there, t0, p_hi, p_lo);
+        uint32_t nan_of[NB];
+        bool any_nan = false;
+        if (masked) {
+            uint32_t all = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t scales[2] = {values.vs[0][b], values.vs[1][b]};
+                nan_of[b] = kv_mend_scales(scales, there, t0, g, max_limit);
+                values.vs[0][b] = scales[0];
+                values.vs[1][b] = scales[1];
+                all |= nan_of[b];
+            }
+            any_nan = any_lane(all != 0u);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t codes[2] = {values.v[0][b], values.v[1][b]}, scales[2] = {values.vs[0][b], values.vs[1][b]};
+            kv_bf16x8 v8[2];
+            kv_v_operands(codes, scales, v8);
+#pragma unroll
+            for (int n2 = 0; n2 < 2; ++n2) multiply_values(v8[n2], b, n2, p_hi, p_lo);
+        }
+        fetch_values(a, values, p, after);
+        if (any_nan) {                                   // rare
+#pragma unroll
+            for (int b = 0; b < NB; ++b) spread_nan(b, or_over_groups(nan_of[b]), t0);
         }
     }
 };
 
 // rounds to the output type and stores elements e0 .. e0 + 7 of a row
-template <int DT>
+template <int DT, bool WIDE = false>
 __device__ __forceinline__ void kv_store8(const KvAttnArgs& a, unsigned short* row, int e0, const float* y) {
     if (e0 >= a.c.head_dim) return;
-    if (a.out_wide) {
-        *reinterpret_cast<u32x4*>(row + e0) = u32x4{Pack<DT>::put(y[0], y[1]), Pack<DT>::put(y[2], y[3]),
-                                                    Pack<DT>::put(y[4], y[5]), Pack<DT>::put(y[6], y[7])};
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e0 + e < a.c.head_dim) row[e0 + e] = (unsigned short)Pack<DT>::put(y[e], y[e]);
+    const u32x4 w = {Pack<DT>::put(y[0], y[1]), Pack<DT>::put(y[2], y[3]), Pack<DT>::put(y[4], y[5]), Pack<DT>::put(y[6], y[7])};
+    if (WIDE || a.out_wide) *reinterpret_cast<u32x4*>(row + e0) = w;
+    else kv_store8_unaligned(row, e0, a.c.head_dim, w);
 }
 __device__ __forceinline__ unsigned short* kv_out_row(const KvAttnArgs& a, int64_t row, int64_t q_head) {
     return a.out + row * a.out_token + q_head * a.out_head;
@@ -414,32 +571,207 @@ __device__ __forceinline__ float kv_lse(float m, float l) {
     return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
-// where the partial results of a workgroup's first (0) or last (1) item lie: columns x (maximum, sum, elements)
+// where the partial results of a workgroup's first (0) or last (1) item lie, by column: elements, and behind all of
+// them maximum and sum
+__device__ __forceinline__ int64_t kv_part_row(const KvAttnArgs& a, int64_t share, int head, int place, int column) {
+    return ((share * a.c.heads + head) * 2 + place) * a.tile_columns + column;
+}
 template <int NB>
-__device__ __forceinline__ float* kv_part(const KvAttnArgs& a, int64_t share, int head, int place, int column) {
-    return a.part + (((share * a.c.heads + head) * 2 + place) * a.tile_columns + column) * (32 * NB + 2);
+__device__ __forceinline__ float* kv_part(const KvAttnArgs& a, int64_t row) { return a.part + row * (32 * NB); }
+template <int NB>
+__device__ __forceinline__ float* kv_part_ml(const KvAttnArgs& a, int64_t row) {
+    return a.part + (int64_t)a.shares * a.c.heads * 2 * a.tile_columns * (32 * NB) + 2 * row;
+}
+
+template <int DT>
+constexpr int kv_terms() { return DT == MXQ_F16 ? 2 : 1; }
+// columns of a wave, in tiles of 16: accumulators and q fill about 160 of the 256 registers that leave two waves a SIMD
+constexpr int kv_prompt_ct(int nb, int terms) {
+    return nb * (8 + 4 * terms) * 4 <= 120 ? 4 : nb * (8 + 4 * terms) * 3 <= (terms == 1 ? 144 : 120) ? 3 : nb * (8 + 4 * terms) * 2 <= 160 ? 2 : 1;
+}
+
+// Items (a request's columns, COLS at a time) differ in the tokens they see, and a grid of items rarely fills the chip
+// evenly.  So the work is numbered through -- an item counts the tokens it sees, in units of 1 / G -- and every workgroup
+// of a head takes an equal stretch of the numbers: an item that a stretch ends in is cut between two of its tiles of 64
+// tokens, and the join kernel adds its parts.  Numbers are closed forms of the group, so a place is found without a table.
+// One workgroup of the decode kernel's launch, which comes first, works the stretches out (kv_plan), the same for every
+// head: in the prompt kernel itself their arithmetic in 64 bits would hold registers that its loop needs.
+struct KvPrompt {
+    int groups;
+    int64_t first;                                       // what group 0 counts; a later one `step` more than the one before
+    int64_t step;
+    __device__ __forceinline__ int64_t begin(int64_t g) const { return g * first + step * (g * (g - 1) / 2); }
+    __device__ __forceinline__ int group_of(int64_t number) const {          // number < begin(groups)
+        int lo = 0, hi = groups;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (begin(mid) <= number) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+};
+__device__ __forceinline__ KvPrompt kv_prompt(const KvAttnArgs& a, const KvSeq& s, int cols) {
+    const int columns = s.fresh * a.group;
+    if (columns == 0 || columns <= a.decode_columns) return KvPrompt{0, 0, 0};
+    const int64_t seen = a.causal ? (s.len > s.fresh ? s.len - s.fresh : 0) : s.keys;
+    return KvPrompt{(columns + cols - 1) / cols, (seen + 64) * a.group + (a.causal ? cols / 2 : 0), a.causal ? cols : 0};
+}
+struct KvStretch {
+    int64_t each, more;
+    int shares;
+    // no stretch is shorter than 256 tokens for an item
+    __device__ __forceinline__ KvStretch(const KvAttnArgs& a, int64_t total) {
+        const int64_t most = total / (256 * a.group);
+        shares = most < 1 ? 1 : most < a.prompt_shares ? (int)most : a.prompt_shares;
+        each = total / shares;
+        more = total - each * shares;
+    }
+    __device__ __forceinline__ int64_t begin(int64_t w) const { return w * each + (w < more ? w : more); }
+    __device__ __forceinline__ int of(int64_t number) const {
+        const int64_t big = more * (each + 1);
+        return number < big ? (int)(number / (each + 1)) : (int)(more + (number - big) / each);
+    }
+};
+// tiles of group g and the first one behind number x (x inside the group's numbers or beyond)
+__device__ __forceinline__ int kv_prompt_tiles(const KvAttnArgs& a, const KvSeq& s, int g, int cols) {
+    const int columns = s.fresh * a.group;
+    const int last = ((g + 1) * cols < columns ? (g + 1) * cols : columns) - 1;
+    return (kv_limit(a, s, last / a.group) + 63) / 64;
+}
+__device__ __forceinline__ int kv_prompt_cut(const KvPrompt& p, int g, int tiles, int64_t x) {
+    const int64_t b = p.begin(g), e = p.begin(g + 1);
+    if (x <= b) return 0;
+    if (x >= e) return tiles;
+    return (int)((double)(x - b) / (double)(e - b) * tiles);
+}
+
+// what kv_plan leaves in the workspace
+struct KvPiece {                                         // of an item, for a workgroup: tiles tile0 .. tile1 - 1
+    int request, group_flags, tile0, tile1;              // flags: 2 the whole item, 1 its second place for parts
+};
+struct KvPlanView {
+    int* head;                                           // items, shares
+    int* items;                                          // of each item: first and last share that it lies in
+    int* shares;                                         // of each share: its first piece, number of pieces
+    KvPiece* pieces;                                     // of item i in share w: at i + w
+    int64_t* first;                                      // of each request: its first number
+    int* item;                                           // .. and its first item
+};
+// (items + shares pieces; 16-byte pieces first)
+__host__ __device__ __forceinline__ int64_t kv_plan_bytes(int64_t items, int64_t shares, int64_t requests) {
+    return 16 * (items + shares) + 8 * requests + 4 * (2 + 2 * items + 2 * shares + requests);
+}
+__device__ __forceinline__ KvPlanView kv_plan_view(const KvAttnArgs& a) {
+    KvPlanView v;
+    v.pieces = reinterpret_cast<KvPiece*>(a.plan);
+    v.first = reinterpret_cast<int64_t*>(v.pieces + a.prompt_items + a.prompt_shares);
+    v.head = reinterpret_cast<int*>(v.first + a.requests);
+    v.items = v.head + 2;
+    v.shares = v.items + 2 * (int64_t)a.prompt_items;
+    v.item = v.shares + 2 * (int64_t)a.prompt_shares;
+    return v;
+}
+__device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* s_wave64, int* s_wave) {
+    const KvPlanView v = kv_plan_view(a);
+    int64_t total = 0;
+    int items = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += TPB) {
+        const int r = r0 + threadIdx.x;
+        KvPrompt p{0, 0, 0};
+        if (r < a.requests) p = kv_prompt(a, kv_seq(a, r), cols);
+        int64_t sum;
+        int group_sum;
+        const int64_t count = p.begin(p.groups), upto = block_scan(count, s_wave64, &sum);
+        const int group_upto = block_scan(p.groups, s_wave, &group_sum);
+        if (r < a.requests) {
+            v.first[r] = total + upto - count;
+            v.item[r] = items + group_upto - p.groups;
+        }
+        total += sum;
+        items += group_sum;
+    }
+    __syncthreads();
+    const KvStretch deal(a, total);
+    if (threadIdx.x == 0) {
+        v.head[0] = items;
+        v.head[1] = total > 0 ? deal.shares : 0;
+    }
+    if (total == 0) return;
+    for (int w = threadIdx.x; w < deal.shares; w += TPB) {
+        const int64_t from = deal.begin(w), to = deal.begin(w + 1);
+        int lo = 0, hi = a.requests;                     // the last request that begins at or before `from` has it
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (v.first[mid] <= from) lo = mid;
+            else hi = mid;
+        }
+        int begun = -1, count = 0;
+        for (int r = lo; r < a.requests; ++r) {
+            const int64_t number = v.first[r];
+            if (number >= to) break;
+            const KvSeq s = kv_seq(a, r);
+            const KvPrompt p = kv_prompt(a, s, cols);
+            if (p.groups == 0) continue;
+            for (int g = from > number ? p.group_of(from - number) : 0; g < p.groups && number + p.begin(g) < to; ++g) {
+                const int tiles = kv_prompt_tiles(a, s, g, cols), item = v.item[r] + g;
+                const int tile0 = kv_prompt_cut(p, g, tiles, from - number), tile1 = kv_prompt_cut(p, g, tiles, to - number);
+                const bool begins = number + p.begin(g) >= from;
+                const bool whole = tile1 - tile0 == tiles && (tiles > 0 || begins);
+                v.pieces[item + w] = KvPiece{r, 4 * g + (whole ? 2 : 0) + (number + p.begin(g) > from ? 1 : 0), tile0, tile1};
+                if (begins) {
+                    v.items[2 * item] = w;
+                    v.items[2 * item + 1] = deal.of(number + p.begin(g + 1) - 1);
+                }
+                if (begun < 0) begun = item + w;
+                ++count;
+            }
+        }
+        v.shares[2 * w] = begun;
+        v.shares[2 * w + 1] = count;
+    }
 }
 
 // ---- few columns -----------------------------------------------------------------------------------------------
-// Units of all requests (each 128 tokens of one column group) are numbered through; workgroup w of W of a head
-// takes the units from floor(w U / W) to floor((w + 1) U / W).
-__device__ __forceinline__ int64_t kv_share_begin(int64_t w, int64_t units, int64_t shares) { return w * units / shares; }
-__device__ __forceinline__ int64_t kv_share_of(int64_t unit, int64_t units, int64_t shares) {
-    return ((unit + 1) * shares - 1) / units;
+// Units of all requests (each 128 tokens of one column group) are numbered through and dealt out to the workgroups of a
+// head in order, as evenly as it goes: the first `more` of them have one unit more than `each`.
+struct KvShares {
+    int each, more;
+    __device__ __forceinline__ KvShares(int units, int shares) : each(units / shares), more(units - units / shares * shares) {}
+    __device__ __forceinline__ int begin(int w) const { return w * each + (w < more ? w : more); }
+    __device__ __forceinline__ int of(int unit) const {
+        const int big = more * (each + 1);
+        return unit < big ? unit / (each + 1) : more + (unit - big) / each;
+    }
+};
+
+// Registers of a wave: accumulators, q, the tiles under way and the rest; the waves that share a SIMD and the tiles
+// that each has under way follow from them.
+constexpr int kv_decode_registers(int nb, int ct, int terms, int depth) {
+    return nb * (8 * ct + 4 * ct * terms + 7 * depth) + 80 + 18 * ct - 8 + 10 * (terms - 1);
 }
+constexpr int kv_decode_depth(int, int, int) { return 1; }
+constexpr int kv_decode_waves(int nb, int ct, int terms) {
+    return kv_decode_registers(nb, ct, terms, 1) <= 126 ? 4 : kv_decode_registers(nb, ct, terms, 1) <= 168 ? 3 : kv_decode_registers(nb, ct, terms, 1) <= 245 && nb != 7 && (nb != 6 || terms == 1) ? 2 : 1;
+}
+// two tiles of columns for one reading of the tokens, where the registers allow it
+constexpr int kv_decode_most_ct(int nb, int terms) { return nb * (23 + 8 * terms) + 100 <= 240 ? 2 : 1; }
 
 template <int DT, int NB, int CT>
-__global__ __launch_bounds__(TPB, NB * CT <= 8 ? 2 : 1)
+__global__ __launch_bounds__(TPB, kv_decode_waves(NB, CT, DT == MXQ_F16 ? 2 : 1))
 void kv_decode_kernel(KvAttnArgs a) {
-    constexpr int NT = DT == MXQ_F16 ? 2 : 1, PB = NB < 4 ? NB : 4, PITCH = 32 * PB + 4;
-    constexpr int CAP = 256;                             // requests scanned at a time
-    static_assert(CAP == TPB, "a thread scans a request");
-    __shared__ int64_t s_wave[TPB / 64];
-    __shared__ int64_t s_begin[CAP];                     // first unit of each request of the scanned stretch
+    constexpr int NT = kv_terms<DT>(), PB = NB < 4 ? NB : 4, PITCH = 32 * PB + 4;
+    __shared__ int s_wave[TPB / 64];
+    __shared__ int s_found[2];                           // the request that the workgroup's units begin in, its first number
     __shared__ float s_ml[4][16][2];
     __shared__ __attribute__((aligned(16))) float s_acc[4][16][PITCH];
+    if (a.plan && blockIdx.x == gridDim.x - 1) {
+        __shared__ int64_t s_wave64[TPB / 64];
+        kv_plan(a, 64 * kv_prompt_ct(NB, NT), s_wave64, s_wave);
+        return;
+    }
     const int head = blockIdx.x % a.c.heads, share = blockIdx.x / a.c.heads;
-    const int wave = threadIdx.x >> 6;
+    const int wave = uniform(threadIdx.x >> 6);
 
     if (a.zero_tail && a.starts) {                       // rows behind the last request of a new output
         int64_t tail = a.starts[a.requests];
@@ -452,61 +784,70 @@ void kv_decode_kernel(KvAttnArgs a) {
         }
     }
 
-    int64_t total = 0;
-    if (!a.whole && a.requests > CAP) {                  // with fewer, the one scan below tells it
-        int64_t mine = 0;
-        for (int r = threadIdx.x; r < a.requests; r += TPB) {
+    // the workgroup's numbers at .. end - 1: units, or with a workgroup for each item (whole) items
+    int at = share, end = share + 1, window = share, number = share;
+    if (!a.direct) {                                     // (direct: one item a request, a workgroup for each)
+        const auto count_of = [&](int r) {
+            if (r >= a.requests) return 0;
             const KvWork w = kv_work(a, kv_seq(a, r));
-            mine += (int64_t)w.units * w.groups;
+            return a.whole ? w.groups : w.count();
+        };
+        int mine = count_of(threadIdx.x), sum, upto = block_scan(mine, s_wave, &sum), total = sum;
+        if (a.requests > TPB) {
+            int rest = 0;
+            for (int r = TPB + threadIdx.x; r < a.requests; r += TPB) rest += count_of(r);
+            total += block_sum(rest, s_wave);
         }
-        total = block_sum(mine, s_wave);
+        if (!a.whole) {
+            const KvShares deal(total, a.shares);
+            at = deal.begin(share);
+            end = deal.begin(share + 1);
+        }
+        if (at >= end || at >= total) return;
+        int before = 0;
+        for (int r0 = 0;; r0 += TPB) {                   // one round for up to 256 requests
+            const int first = before + upto - mine;
+            if (first <= at && at < first + mine) {
+                s_found[0] = r0 + threadIdx.x;
+                s_found[1] = first;
+            }
+            before += sum;
+            if (at < before) break;
+            mine = count_of(r0 + TPB + threadIdx.x);
+            upto = block_scan(mine, s_wave, &sum);
+        }
+        __syncthreads();
+        window = uniform(s_found[0]);
+        number = uniform(s_found[1]);
     }
-    int64_t before = 0, begin = 0, end = 0;
-    bool known = false;
-    for (int r0 = 0; r0 < a.requests; r0 += CAP) {
-        KvWork w{0, 0};
-        if (r0 + (int)threadIdx.x < a.requests) w = kv_work(a, kv_seq(a, r0 + threadIdx.x));
-        // with a workgroup for each item the numbers run over the items, whatever their units
-        const int64_t count = a.whole ? (int64_t)w.groups : (int64_t)w.units * w.groups;
-        int64_t sum;
-        const int64_t upto = block_scan(count, s_wave, &sum);
-        __syncthreads();
-        s_begin[threadIdx.x] = before + upto - count;
-        __syncthreads();
-        if (!known) {
-            if (a.requests <= CAP) total = sum;
-            begin = a.whole ? share : kv_share_begin(share, total, a.shares);
-            end = a.whole ? share + 1 : kv_share_begin(share + 1, total, a.shares);
-            known = true;
+    const int first_number = at;
+    // 64 requests at a time sit in the lanes
+    const int lane = threadIdx.x & 63;
+    for (; at < end && window < a.requests; window += 64) {
+        KvSeq in_lane{0, 0, 0, 0};
+        KvWork work_in_lane{0, 0};
+        if (window + lane < a.requests) {
+            in_lane = kv_seq(a, window + lane);
+            work_in_lane = kv_work(a, in_lane);
         }
-        const int64_t stretch_end = before + sum;
-        int64_t at = begin > before ? begin : before;
-        // the request of unit `at`: the last one that begins at or before it (those without units share its number
-        // with the next one, so the last is the one that has it)
-        int lo = 0, hi = CAP;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (s_begin[mid] <= at && r0 + mid < a.requests) lo = mid;
-            else hi = mid;
-        }
-        for (int k = lo; at < end && at < stretch_end; ++k) {
-            const int r = r0 + k;
-            const KvSeq s = kv_seq(a, r);
-            const KvWork wk = kv_work(a, s);
+        const int last_lane = 63 < a.requests - 1 - window ? 63 : a.requests - 1 - window;
+        for (int k = 0; k <= last_lane && at < end; ++k) {
+            const KvWork wk{__builtin_amdgcn_readlane(work_in_lane.units, k), __builtin_amdgcn_readlane(work_in_lane.groups, k)};
             if (wk.groups == 0) continue;
-            const int64_t req0 = s_begin[k];
+            const int r = window + k;
+            const KvSeq s{__builtin_amdgcn_readlane(in_lane.row0, k), __builtin_amdgcn_readlane(in_lane.fresh, k),
+                          __builtin_amdgcn_readlane(in_lane.len, k), __builtin_amdgcn_readlane(in_lane.keys, k)};
             const int per = a.whole ? 1 : wk.units;
-            for (; at < end && at < req0 + (int64_t)per * wk.groups;) {
-                const int grp = (int)((at - req0) / per);
-                const int64_t item0 = req0 + (int64_t)grp * per;
-                const int64_t stop = end < item0 + per ? end : item0 + per;
-                const int u0 = a.whole ? 0 : (int)(at - item0), u1 = a.whole ? wk.units : (int)(stop - item0);
+            for (int grp = (at - number) / per; grp < wk.groups && at < end; ++grp) {
+                const int item0 = number + grp * per;
+                const int stop = end < item0 + per ? end : item0 + per;
+                const int u0 = a.whole ? 0 : at - item0, u1 = a.whole ? wk.units : stop - item0;
                 const bool complete = u0 == 0 && u1 == wk.units;
-                const int place = item0 > begin ? 1 : 0;
+                const int place = u0 == 0 && !complete && at != first_number ? 1 : 0;
                 const int c0 = grp * 16 * CT, columns = s.fresh * a.group;
                 KvWave<NB, CT, NT, 2> wv;
-                wv.begin(a, s, head, c0);
-                wv.walk(a, r, 4 * u0 + wave, 4 * u1, 4);
+                wv.begin(a, s, head, c0, reinterpret_cast<unsigned short*>(&s_acc[wave][0][0]));
+                wv.template walk<kv_decode_depth(NB, CT, NT)>(a, r, head, 4 * u0 + wave, 4 * u1, 4);
                 // join the four waves: one tile of columns and up to four blocks at a time
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
@@ -522,7 +863,8 @@ void kv_decode_kernel(KvAttnArgs a) {
 #pragma unroll
                         for (int b = 0; b < PB; ++b)
                             if (b < nb) {
-                                const kv_f32x4 even = wv.acc[ct][b0 + b][0], odd = wv.acc[ct][b0 + b][1];
+                                const int at_b = b0 + b < NB ? b0 + b : 0;
+                                const kv_f32x4 even = wv.acc[ct][at_b][0], odd = wv.acc[ct][at_b][1];
                                 float* dst = &s_acc[wave][wv.i16][32 * b + 8 * wv.g];
                                 *reinterpret_cast<kv_f32x4*>(dst) = kv_f32x4{even[0], odd[0], even[1], odd[1]};
                                 *reinterpret_cast<kv_f32x4*>(dst + 4) = kv_f32x4{even[2], odd[2], even[3], odd[3]};
@@ -532,7 +874,7 @@ void kv_decode_kernel(KvAttnArgs a) {
                         for (int e = threadIdx.x; e < 64 * nb; e += TPB) {
                             const int col = e / (4 * nb), d0 = e % (4 * nb) * 8, c = c0 + 16 * ct + col;
                             if (c >= columns) continue;
-                            float top = -__builtin_inff();
+                            float top = KV_NOTHING;
 #pragma unroll
                             for (int w4 = 0; w4 < 4; ++w4) top = __builtin_fmaxf(top, s_ml[w4][col][0]);
                             float sum_l = 0.0f, y[8];
@@ -540,8 +882,7 @@ void kv_decode_kernel(KvAttnArgs a) {
                             for (int x = 0; x < 8; ++x) y[x] = 0.0f;
 #pragma unroll
                             for (int w4 = 0; w4 < 4; ++w4) {
-                                const float mw = s_ml[w4][col][0];
-                                const float f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
+                                const float f = __builtin_amdgcn_exp2f(s_ml[w4][col][0] - top);
                                 sum_l += s_ml[w4][col][1] * f;
 #pragma unroll
                                 for (int x = 0; x < 8; ++x) y[x] += s_acc[w4][col][d0 + x] * f;
@@ -555,38 +896,100 @@ void kv_decode_kernel(KvAttnArgs a) {
                                 kv_store8<DT>(a, kv_out_row(a, row, qh), 32 * b0 + d0, y);
                                 if (a.lse && b0 == 0 && d0 == 0) a.lse[row * a.c.heads * a.group + qh] = kv_lse(top, sum_l);
                             } else {
-                                float* part = kv_part<NB>(a, share, head, place, 16 * ct + col);
-                                if (b0 == 0 && d0 == 0) {
-                                    part[0] = top;
-                                    part[1] = sum_l;
-                                }
-#pragma unroll
-                                for (int x = 0; x < 8; ++x) part[2 + 32 * b0 + d0 + x] = y[x];
+                                const int64_t part = kv_part_row(a, share, head, place, 16 * ct + col);
+                                if (b0 == 0 && d0 == 0)
+                                    *reinterpret_cast<kv_f32x2*>(kv_part_ml<NB>(a, part)) = kv_f32x2{top, sum_l};
+                                kv_f32x4* dst = reinterpret_cast<kv_f32x4*>(kv_part<NB>(a, part) + 32 * b0 + d0);
+                                dst[0] = kv_f32x4{y[0], y[1], y[2], y[3]};
+                                dst[1] = kv_f32x4{y[4], y[5], y[6], y[7]};
                             }
                         }
                     }
                 }
                 at = stop;
             }
+            number += per * wk.groups;
         }
-        before = stretch_end;
-        if (before >= end) break;                        // uniform over the workgroup
     }
 }
 
-// One workgroup for each row and query head: adds the parts of requests that crossed workgroups, in their order.
+template <int NB>
+__device__ __forceinline__ float* kv_prompt_part(const KvAttnArgs& a, int64_t row) { return a.prompt_part + row * (32 * NB); }
+template <int NB, int COLS>
+__device__ __forceinline__ float* kv_prompt_part_ml(const KvAttnArgs& a, int64_t row) {
+    return a.prompt_part + (int64_t)a.prompt_shares * a.c.heads * 2 * COLS * (32 * NB) + 2 * row;
+}
+
+// 16 columns of an item: adds its parts, in their order, if it was cut.
+template <int DT, int NB, int CT>
+__device__ __forceinline__ void kv_prompt_join(const KvAttnArgs& a, int block) {
+    constexpr int COLS = 64 * CT, DP = 32 * NB;
+    const int head = block % a.c.heads, sixteen = block / a.c.heads % (4 * CT), item = block / a.c.heads / (4 * CT);
+    const KvPlanView plan = kv_plan_view(a);
+    if (plan.head[1] == 0 || item >= plan.head[0]) return;
+    const int w0 = plan.items[2 * item], w1 = plan.items[2 * item + 1];
+    if (w0 == w1 && a.out_wide) return;
+    const KvPiece first = plan.pieces[item + w0];
+    const int grp = first.group_flags >> 2;
+    const KvSeq s = kv_seq(a, first.request);
+    const int columns = s.fresh * a.group;
+    for (int e = threadIdx.x; e < 16 * (DP / 8); e += TPB) {
+        const int col = 16 * sixteen + e / (DP / 8), d0 = e % (DP / 8) * 8, c = grp * COLS + col;
+        if (c >= columns) continue;
+        float m = KV_NOTHING, l = 0.0f, y[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) y[x] = 0.0f;
+        bool cut = false;
+        for (int w = w0; w <= w1; ++w) {
+            const KvPiece piece = plan.pieces[item + w];
+            if (piece.group_flags & 2 ? a.out_wide != 0 : piece.tile0 == piece.tile1) continue;   // written already; nothing done
+            cut = true;
+            const int64_t part = (((int64_t)w * a.c.heads + head) * 2 + (piece.group_flags & 1)) * COLS + col;
+            const kv_f32x2 ml = *reinterpret_cast<const kv_f32x2*>(kv_prompt_part_ml<NB, COLS>(a, part));
+            const kv_f32x4* v = reinterpret_cast<const kv_f32x4*>(kv_prompt_part<NB>(a, part) + d0);
+            const kv_f32x4 lo = v[0], hi = v[1];
+            const float up = __builtin_fmaxf(m, ml[0]);
+            const float f = __builtin_amdgcn_exp2f(m - up), fp = __builtin_amdgcn_exp2f(ml[0] - up);
+            m = up;
+            l = l * f + ml[1] * fp;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                y[x] = y[x] * f + lo[x] * fp;
+                y[x + 4] = y[x + 4] * f + hi[x] * fp;
+            }
+        }
+        if (!cut) continue;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) y[x] *= inv;
+        const int64_t q_row = s.row0 + c / a.group, qh = (int64_t)head * a.group + c % a.group;
+        kv_store8<DT>(a, kv_out_row(a, q_row, qh), d0, y);
+        if (a.lse && d0 == 0) a.lse[q_row * a.c.heads * a.group + qh] = kv_lse(m, l);
+    }
+}
+
+// One workgroup for each row and query head: adds the parts of a request that crossed workgroups, in their order.
+// Behind these workgroups: those of the prompt kernel's cut items.
 template <int DT, int NB>
 __global__ __launch_bounds__(TPB) void kv_join_kernel(KvAttnArgs a) {
     constexpr int DP = 32 * NB, LANES = DP / 4, ROWS = TPB / LANES;          // 4 elements a thread, ROWS parts at a time
-    __shared__ int64_t s_wave[TPB / 64];
+    __shared__ int s_wave[TPB / 64];
     __shared__ int s_request;
-    __shared__ float s_ml[ROWS][2];
-    __shared__ float s_acc[ROWS][DP];
+    __shared__ float s_weight[KV_MAX_SHARES];
+    __shared__ float s_top[TPB / 64], s_sum[TPB / 64];
+    __shared__ kv_f32x4 s_acc[ROWS][LANES];
+    if ((int)blockIdx.x >= a.join_blocks) {
+        kv_prompt_join<DT, NB, kv_prompt_ct(NB, kv_terms<DT>())>(a, (int)blockIdx.x - a.join_blocks);
+        return;
+    }
     const int q_heads = a.c.heads * a.group;
-    const int64_t row = blockIdx.x / q_heads;
     const int qh = blockIdx.x % q_heads, head = qh / a.group;
+    int64_t row = blockIdx.x / q_heads;
     int r = (int)row;
-    if (a.starts) {
+    if (a.join_rows) {                                   // the first rows of each request: others are the prompt kernel's
+        r = (int)(row / a.join_rows);
+        row -= (int64_t)r * a.join_rows;
+    } else if (a.starts) {
         if (threadIdx.x == 0) s_request = -1;
         __syncthreads();
         for (int k = threadIdx.x; k < a.requests; k += TPB) {
@@ -594,117 +997,254 @@ __global__ __launch_bounds__(TPB) void kv_join_kernel(KvAttnArgs a) {
             if (s.row0 <= row && row < s.row0 + s.fresh) s_request = k;
         }
         __syncthreads();
-        r = s_request;
+        r = uniform(s_request);
         if (r < 0) return;
     }
     const KvSeq s = kv_seq(a, r);
     const KvWork wk = kv_work(a, s);
-    if (wk.groups == 0) return;                          // the prompt kernel's
-    int64_t mine = 0, mine_before = 0;
+    if (wk.groups == 0) return;
+    if (a.join_rows) {
+        if (row >= s.fresh) return;
+        row += s.row0;
+    }
+    int mine = 0, mine_before = 0;
     for (int k = threadIdx.x; k < a.requests; k += TPB) {
-        const KvWork w = kv_work(a, kv_seq(a, k));
-        const int64_t n = (int64_t)w.units * w.groups;
+        const int n = kv_work(a, kv_seq(a, k)).count();
         mine += n;
         if (k < r) mine_before += n;
     }
-    const int64_t total = block_sum(mine, s_wave), before = block_sum(mine_before, s_wave);
+    const int total = block_sum(mine, s_wave), before = block_sum(mine_before, s_wave);
     const int c = (int)(row - s.row0) * a.group + qh % a.group, grp = c / a.tile_columns, col = c % a.tile_columns;
-    const int64_t item0 = before + (int64_t)grp * wk.units, item1 = item0 + wk.units;
-    const int64_t w0 = kv_share_of(item0, total, a.shares), w1 = kv_share_of(item1 - 1, total, a.shares);
+    const int item0 = before + grp * wk.units, item1 = item0 + wk.units;
+    const KvShares deal(total, a.shares);
+    const int w0 = deal.of(item0), w1 = deal.of(item1 - 1);
     if (w0 == w1) return;                                // written by the workgroup that had all of it
-    const int lane = threadIdx.x % LANES, part_row = threadIdx.x / LANES;
-    float m = -__builtin_inff(), l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (part_row < ROWS) {
-        for (int64_t w = w0 + part_row; w <= w1; w += ROWS) {
-            const int64_t begin = kv_share_begin(w, total, a.shares);
-            if (begin == kv_share_begin(w + 1, total, a.shares)) continue;   // more workgroups than units: left nothing
-            const int place = item0 > begin ? 1 : 0;
-            const float* part = kv_part<NB>(a, w, head, place, col);
-            const float pm = part[0], pl = part[1];
-            if (pm == -__builtin_inff()) continue;       // nothing seen there
-            const float up = __builtin_fmaxf(m, pm);
-            const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - up), fp = __builtin_amdgcn_exp2f(pm - up);
-            l = l * f + pl * fp;
+    const int parts = w1 - w0 + 1;
+    const auto part_row = [&](int k) {
+        return kv_part_row(a, w0 + k, head, item0 > deal.begin(w0 + k) ? 1 : 0, col);
+    };
+    // maxima and sums of all parts at once
+    float m = KV_NOTHING;
+    for (int k = threadIdx.x; k < parts; k += TPB) {
+        const float pm = kv_part_ml<NB>(a, part_row(k))[0];                  // (none between w0 and w1 is without a unit)
+        s_weight[k] = pm;
+        m = __builtin_fmaxf(m, pm);
+    }
+    for (int d = 32; d; d >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d, 64));
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const float top = __builtin_fmaxf(__builtin_fmaxf(s_top[0], s_top[1]), __builtin_fmaxf(s_top[2], s_top[3]));
+    float l = 0.0f;
+    for (int k = threadIdx.x; k < parts; k += TPB) {
+        const float w = __builtin_amdgcn_exp2f(s_weight[k] - top);
+        s_weight[k] = w;
+        l += kv_part_ml<NB>(a, part_row(k))[1] * w;
+    }
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d, 64);
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = l;
+    __syncthreads();
+    const float sum_l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES;
+    kv_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (first < ROWS) {
+        int k = first;
+        for (; k + 3 * ROWS < parts; k += 4 * ROWS) {    // four loads under way
+            kv_f32x4 v[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) y[x] = y[x] * f + part[2 + 4 * lane + x] * fp;
-            m = up;
-        }
-        if (lane == 0) {
-            s_ml[part_row][0] = m;
-            s_ml[part_row][1] = l;
-        }
+            for (int x = 0; x < 4; ++x) v[x] = reinterpret_cast<const kv_f32x4*>(kv_part<NB>(a, part_row(k + x * ROWS)))[lane];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s_acc[part_row][4 * lane + x] = y[x];
+            for (int x = 0; x < 4; ++x) y += v[x] * s_weight[k + x * ROWS];
+        }
+        for (; k < parts; k += ROWS) y += reinterpret_cast<const kv_f32x4*>(kv_part<NB>(a, part_row(k)))[lane] * s_weight[k];
+        s_acc[first][lane] = y;
     }
     __syncthreads();
-    float top = -__builtin_inff(), sum_l = 0.0f;
-    for (int k = 0; k < ROWS; ++k) top = __builtin_fmaxf(top, s_ml[k][0]);
-    for (int k = 0; k < ROWS; ++k)
-        if (s_ml[k][0] != -__builtin_inff()) sum_l += s_ml[k][1] * __builtin_amdgcn_exp2f(s_ml[k][0] - top);
     const float inv = sum_l == 0.0f ? 0.0f : 1.0f / sum_l;
     unsigned short* o = kv_out_row(a, row, qh);
     for (int d = threadIdx.x; d < a.c.head_dim; d += TPB) {
         float v = 0.0f;
-        for (int k = 0; k < ROWS; ++k)
-            if (s_ml[k][0] != -__builtin_inff()) v += s_acc[k][d] * __builtin_amdgcn_exp2f(s_ml[k][0] - top);
+        for (int k = 0; k < ROWS; ++k) v += s_acc[k][d >> 2][d & 3];
         o[d] = (unsigned short)Pack<DT>::put(v * inv, 0.0f);
     }
     if (a.lse && threadIdx.x == 0) a.lse[row * q_heads + qh] = kv_lse(top, sum_l);
 }
 
 // ---- many columns ----------------------------------------------------------------------------------------------
-// A workgroup takes 4 x 16 CT columns of a request, a quarter for each wave; the waves do not meet.
-constexpr int kv_prompt_ct(int nb) { return nb <= 4 ? 4 : 2; }
+// A workgroup takes 4 x 16 CT columns of a request (an item), a quarter for each wave, and walks over 64 tokens at a time: the
+// waves decode their shares of K and V to bf16 once, into LDS and in the order of the operands (a lane reads its 16
+// bytes next to its neighbours'), and all of them multiply from there.  Two buffers: the tile ahead is decoded, the
+// one behind it loaded, while a tile is multiplied; one barrier a tile.
+template <int NB>
+struct KvShare {                                         // what a lane loads of 64 tokens for its wave to decode
+    static constexpr int VB = (NB + 1) / 2;
+    uint32_t k[NB], ks[kv_k_scales<NB>()];               // K: 16 tokens, all blocks
+    uint32_t v[VB][2], vs[VB][2];                        // V: 32 tokens, every other block
+};
+
 template <int DT, int NB, int CT>
-__global__ __launch_bounds__(TPB, NB * CT <= 8 ? 2 : 1) void kv_prompt_kernel(KvAttnArgs a) {
-    constexpr int NT = DT == MXQ_F16 ? 2 : 1, NP = DT == MXQ_F16 ? 2 : 1, COLS = 64 * CT;
-    __shared__ int64_t s_wave[TPB / 64];
-    __shared__ int s_request, s_tile;
-    const int head = blockIdx.x % a.c.heads;
-    const int64_t want = blockIdx.x / a.c.heads;
-    if (threadIdx.x == 0) s_request = -1;
-    int64_t before = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += TPB) {
-        int64_t n = 0, sum;
-        const int r = r0 + threadIdx.x;
-        if (r < a.requests) {
-            const int64_t columns = (int64_t)kv_seq(a, r).fresh * a.group;
-            if (columns > a.decode_columns) n = (columns + COLS - 1) / COLS;
-        }
-        const int64_t upto = before + block_scan(n, s_wave, &sum);
-        if (want < upto && want >= upto - n) {
-            s_request = r;
-            s_tile = (int)(want - (upto - n));
-        }
-        before += sum;
-    }
-    __syncthreads();
-    const int r = s_request;
-    if (r < 0) return;
-    const KvSeq s = kv_seq(a, r);
-    const int columns = s.fresh * a.group;
-    // the tiles that see the most come first
-    const int c0 = ((columns + COLS - 1) / COLS - 1 - s_tile) * COLS + (threadIdx.x >> 6) * (16 * CT);
-    if (c0 >= columns) return;
-    KvWave<NB, CT, NT, NP> wv;
-    wv.begin(a, s, head, c0);
-    wv.walk(a, r, 0, 0x7FFFFFFF / 32, 1);
+__global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
+    constexpr int NT = kv_terms<DT>(), NP = kv_terms<DT>(), COLS = 64 * CT, VB = KvShare<NB>::VB;
+    using Wave = KvWave<NB, CT, NT, NP>;
+    __shared__ uint32_t s_nan[2][2][NB];                 // masked tiles: tokens with a NaN block, by half of 32 tokens
+    __shared__ u32x4 s_k[2][4 * NB][64], s_v[2][4 * NB][64];                 // [buffer][operand][lane]
+    const int head = blockIdx.x % a.c.heads, w = blockIdx.x / a.c.heads;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g4 = lane >> 4, i16 = lane & 15;
+    const KvPlanView plan = kv_plan_view(a);
+    if (w >= plan.head[1]) return;
+    const int piece0 = uniform(plan.shares[2 * w]), piece1 = piece0 + uniform(plan.shares[2 * w + 1]);
+    for (int at_piece = piece0; at_piece < piece1; ++at_piece) {
+        const KvPiece piece = plan.pieces[at_piece];
+        const int r = uniform(piece.request), flags = uniform(piece.group_flags), grp = flags >> 2;
+        const int tile0 = uniform(piece.tile0), tile1 = uniform(piece.tile1);
+        if (tile0 == tile1 && !(flags & 2)) continue;
+        const bool complete = (flags & 2) && a.out_wide;        // (rows that are not aligned are the join kernel's)
+        const KvSeq in_lanes = kv_seq(a, r);
+        const KvSeq s{uniform(in_lanes.row0), uniform(in_lanes.fresh), uniform(in_lanes.len), uniform(in_lanes.keys)};
+        const int columns = s.fresh * a.group;
+        const int wg_c0 = grp * COLS, c0 = wg_c0 + wave * (16 * CT);
+        const int wg_last = (wg_c0 + COLS < columns ? wg_c0 + COLS : columns) - 1;
+        const int wg_min = kv_limit(a, s, wg_c0 / a.group), wg_max = kv_limit(a, s, wg_last / a.group);
+        const bool works = c0 < columns;         // uniform over the wave
+        Wave wv;
+        wv.begin(a, s, head, works ? c0 : wg_c0, reinterpret_cast<unsigned short*>(&s_k[0][0][0]) + wave * (16 * 32 * NB));
+        const int half = wave & 1;
+        const int* row = a.table + (int64_t)r * a.table_stride;
+        typename Wave::Spot spots;                           // lane: 16 tokens of the next sixteen tiles
+        uint64_t there_mask = 0;
+        wv.place(a);
+        KvShare<NB> share;
+        int share_there = 0;                                 // which of the loaded tile's four pages exist
+        const auto load = [&](int tile) {
+            const int at = 4 * ((tile - tile0) & 15);
+            if (at == 0) {
+                spots = Wave::spot(a, row, head, 4 * tile + lane, (wg_max + 15) / 16);
+                there_mask = __ballot(spots.there);
+            }
+            share_there = (int)(there_mask >> at) & 15;
+            {
+                const __amdgpu_buffer_rsrc_t source = Wave::lane_codes(a, spots, at + wave);
+                const int scales = __builtin_amdgcn_readlane(spots.scales, at + wave);
+                load_dwords<NB>(source, wv.at_k, 0, share.k);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-        const float l = sum_over_groups(wv.l[ct]);
-        const int c = c0 + 16 * ct + wv.i16;
-        if (c >= columns) continue;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int64_t row = s.row0 + c / a.group, qh = (int64_t)head * a.group + c % a.group;
-        unsigned short* o = kv_out_row(a, row, qh);
+                for (int k = 0; k < kv_k_scales<NB>(); ++k) share.ks[k] = __builtin_amdgcn_raw_buffer_load_b8(source, wv.at_ks[k], scales, 0);
+            }
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float y[8];
+            for (int j = 0; j < 2; ++j) {
+                const int from = at + 2 * half + j;
+                const __amdgpu_buffer_rsrc_t source = Wave::lane_codes(a, spots, from);
+                const int scales = __builtin_amdgcn_readlane(spots.scales, from);
 #pragma unroll
-            for (int x = 0; x < 8; ++x) y[x] = wv.acc[ct][b][x & 1][x >> 1] * inv;
-            kv_store8<DT>(a, o, 32 * b + 8 * wv.g, y);
+                for (int x = 0; x < VB; ++x) {
+                    int b = (wave >> 1) + 2 * x;
+                    if (b > NB - 1) b = NB - 1;              // (an odd NB: two waves have one block less)
+                    share.v[x][j] = __builtin_amdgcn_raw_buffer_load_b32(source, wv.at_v, 4 * b, 0);
+                    share.vs[x][j] = __builtin_amdgcn_raw_buffer_load_b32(source, wv.at_vs, scales + 4 * b, 0);
+                }
+            }
+        };
+        int there_bits[2] = {0, 0};                          // by buffer: which of the tile's four pages exist
+        const auto decode = [&](int tile, int buffer) {
+#pragma unroll
+            for (int st = 0; st < NB; ++st)
+                s_k[buffer][wave * NB + st][lane] =
+                    __builtin_bit_cast(u32x4, kv_k_operand(share.k[st], kv_k_scale<NB>(share.ks, g4, st)));
+            there_bits[buffer] = share_there;
+            const bool masked = 64 * tile + 64 > wg_min || share_there != 15;
+            const bool there2[2] = {(share_there >> (2 * half) & 1) != 0, (share_there >> (2 * half + 1) & 1) != 0};
+#pragma unroll
+            for (int x = 0; x < VB; ++x) {
+                const int b = (wave >> 1) + 2 * x;
+                if (b < NB) {
+                    uint32_t scales[2] = {share.vs[x][0], share.vs[x][1]};
+                    if (masked) {
+                        const uint32_t nan = or_over_groups(kv_mend_scales(scales, there2, 64 * tile + 32 * half, g4, wg_max));
+                        if (lane == 0) s_nan[buffer][half][b] = nan;
+                    }
+                    const uint32_t codes[2] = {share.v[x][0], share.v[x][1]};
+                    kv_bf16x8 v8[2];
+                    kv_v_operands(codes, scales, v8);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) s_v[buffer][(half * NB + b) * 2 + n][lane] = __builtin_bit_cast(u32x4, v8[n]);
+                }
+            }
+        };
+
+        if (tile0 < tile1) {
+            load(tile0);
+            decode(tile0, 0);
+            if (tile0 + 1 < tile1) load(tile0 + 1);
         }
-        if (a.lse && wv.g == 0) a.lse[row * a.c.heads * a.group + qh] = kv_lse(wv.m[ct], l);
+        __syncthreads();
+        for (int tile = tile0; tile < tile1; ++tile) {
+            const int buffer = (tile - tile0) & 1;
+            if (tile + 1 < tile1) {
+                decode(tile + 1, buffer ^ 1);
+                if (tile + 2 < tile1) load(tile + 2);
+            }
+            if (works && 64 * tile < wv.max_limit) {
+                const bool wg_masked = 64 * tile + 64 > wg_min || there_bits[buffer] != 15;
+                // (a loop, not unrolled: both halves at once need registers that are not there)
+#pragma nounroll
+                for (int h = 0; h < 2; ++h) {
+                    const int t0 = 64 * tile + 32 * h;
+                    kv_f32x4 sc[CT][2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int st = 0; st < NB; ++st)
+                            wv.multiply_keys(__builtin_bit_cast(kv_bf16x8, s_k[buffer][(2 * h + j) * NB + st][lane]), j, st, sc);
+                    const bool there[2] = {(there_bits[buffer] >> (2 * h) & 1) != 0, (there_bits[buffer] >> (2 * h + 1) & 1) != 0};
+                    const bool masked = t0 + 32 > wv.min_limit || !there[0] || !there[1];
+                    uint32_t p_hi[CT][4], p_lo[CT][4];
+                    wv.probabilities(a, sc, masked, there, t0, p_hi, p_lo);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            wv.multiply_values(__builtin_bit_cast(kv_bf16x8, s_v[buffer][(h * NB + b) * 2 + n][lane]), b, n, p_hi, p_lo);
+                    if (wg_masked) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const uint32_t of = s_nan[buffer][h][b];
+                            if (any_lane(of != 0u)) wv.spread_nan(b, of, t0);
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (!works) continue;
+        // addresses below are worked out here: known before, they would be kept in registers through the loop above
+        const int g_out = here_only(g4), i_out = here_only(i16);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            const float l = sum_over_groups(wv.l[ct]);
+            const int c = c0 + 16 * ct + i_out;
+            if (c >= columns) continue;
+            if (complete) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int64_t q_row = s.row0 + c / a.group, qh = (int64_t)head * a.group + c % a.group;
+                unsigned short* o = kv_out_row(a, q_row, qh);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float y[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) y[x] = wv.acc[ct][b][x & 1][x >> 1] * inv;
+                    kv_store8<DT, true>(a, o, 32 * b + 8 * g_out, y);
+                }
+                if (a.lse && g_out == 0) a.lse[q_row * a.c.heads * a.group + qh] = kv_lse(wv.m[ct], l);
+            } else {
+                const int64_t part = (((int64_t)w * a.c.heads + head) * 2 + (flags & 1)) * COLS + (c - wg_c0);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    kv_f32x4* dst = reinterpret_cast<kv_f32x4*>(kv_prompt_part<NB>(a, part) + 32 * b + 8 * g_out);
+                    const kv_f32x4 even = wv.acc[ct][b][0], odd = wv.acc[ct][b][1];
+                    dst[0] = kv_f32x4{even[0], odd[0], even[1], odd[1]};
+                    dst[1] = kv_f32x4{even[2], odd[2], even[3], odd[3]};
+                }
+                if (g_out == 0) *reinterpret_cast<kv_f32x2*>(kv_prompt_part_ml<NB, COLS>(a, part)) = kv_f32x2{wv.m[ct], l};
+            }
+        }
     }
 }
 

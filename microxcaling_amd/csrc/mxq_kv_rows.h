@@ -69,7 +69,7 @@ __global__ __launch_bounds__(TPB) void kv_block_tables_kernel(KvTablesArgs a) {
         const int64_t start = tokens + block_scan(q.fresh, s_wave, &token_sum) - q.fresh;
         const int64_t page = pages + block_scan(q.fresh_pages, s_wave, &page_sum) - q.fresh_pages;
         const bool here = q.fresh > 0 && start < t1 && start + q.fresh > t0;
-        const int64_t at = listed + block_scan(here ? 1 : 0, s_wave, &list_sum) - 1;
+        const int64_t at = listed + block_scan((int64_t)(here ? 1 : 0), s_wave, &list_sum) - 1;
         if (here) {
             s_start[at] = start;
             s_page[at] = page;
@@ -129,9 +129,35 @@ __global__ __launch_bounds__(TPB) void kv_block_tables_kernel(KvTablesArgs a) {
 // quantize and store; read back
 // ================================================================================================================
 // A lane owns 8 elements of a block (a dword of codes): lane bits 0-1 the token of four, 2-3 the quarter j of the
-// block.  K's dword goes out as it is.  Of V the four lanes of a quad hold the bytes (i = 4 j .. 4 j + 3) of four
-// tokens; where these tokens are the four of one V tile (every tile of a prompt), they trade bytes and store a
-// dword each, otherwise (decoding steps) four bytes.  Bound by memory for prompts, by latency for single tokens.
+// block; a group of 16 lanes keeps its head, K or V, and block, and goes through the groups of four tokens.  K's dword
+// goes out as it is.  Of V the four lanes of a quad hold the bytes (i = 4 j .. 4 j + 3) of four tokens; where these
+// tokens are the four of one V tile (every tile of a prompt), they trade bytes and store a dword each, otherwise
+// (decoding steps) four bytes.  Bound by memory for prompts, by latency for single tokens.
+//
+// Rounding half away from zero with v_cvt_scalef32_pk_fp4_f32, which rounds half to even: values are moved a little
+// further from zero first, so that what lies on a border between two codes lies above it, and nothing else crosses one.
+//   bf16: times 1 + 2^-8 + 2^-15.  A border is half of a 2-bit significand's step; the largest bf16 below one of them is
+//     2^-7 of it or more below (2^-8 above a power of two: all but the first border are), except below the first
+//     border 1/4, where 1/4 - 2^-10 is the very value that the bf16 sum with one half carries over it.
+//   fp32 (and fp16 widened): the low 8 bits become 0x80, which puts a border above itself and keeps everything below it
+//     below; 2^-26 is added first, which lets the one value do the same that the fp32 sum with one half carries over.
+// That replaces 14 instructions an element by 3 or 6: 16384 rows of 8 heads of 128 took 46 us with them.
+template <int DT>
+struct KvNudge {
+    static __device__ __forceinline__ float inverse(float inv_scale) { return inv_scale; }
+    static __device__ __forceinline__ float apply(float x, float inv) {
+        const float a = x * inv;
+        const uint32_t away = (mxq_bits(__builtin_fabsf(a) + 1.4901161193847656e-08f) & 0xFFFFFF00u) | 0x80u;
+        return mxq_float(away | (mxq_bits(a + 0.0f) & 0x80000000u));         // (-0 is +0)
+    }
+};
+template <>
+struct KvNudge<MXQ_BF16> {
+    static __device__ __forceinline__ float inverse(float inv_scale) { return inv_scale * 1.003936767578125f; }
+    // + 1.004 x 2^-134: what bf16 would round to zero, -0 among it, becomes +0
+    static __device__ __forceinline__ float apply(float x, float inv) { return __builtin_fmaf(x, inv, 4.610e-41f); }
+};
+
 struct KvRowsArgs {
     const void* k;
     const void* v;
@@ -151,8 +177,8 @@ __device__ __forceinline__ KvPlace kv_place(const KvCache& c, int64_t slot, int 
     KvPlace p{false, nullptr, 0};
     if (slot < 0) return p;
     int64_t page;
-    if (slot < 0x100000000LL) {                          // a 32-bit division is a fraction of a 64-bit one
-        page = (uint32_t)slot / (uint32_t)c.page_size;
+    if (slot < 0x100000000LL) {
+        page = kv_page_of(c, (uint32_t)slot);
         p.off = (int)((uint32_t)slot - (uint32_t)page * (uint32_t)c.page_size);
     } else {
         page = slot / c.page_size;
@@ -183,20 +209,37 @@ __device__ __forceinline__ bool quad_is_tile(int64_t slot, int me) {
     return (quad_lane<0>(ok) & quad_lane<1>(ok) & quad_lane<2>(ok) & quad_lane<3>(ok)) != 0u;
 }
 
-template <int DT, int RMODE, bool ZONE_ELEM, bool DIRECT>
+// the unit of a group of 16 lanes, and the groups of four tokens that it goes through: neighbouring ones, so that the
+// lines that their scales share are completed in one L2
+struct KvUnit {
+    int head, is_v, b;
+    int64_t quad, end;
+};
+__device__ __forceinline__ KvUnit kv_unit(const KvCache& c, int64_t tokens) {
+    const int units = c.heads * 2 * c.nb, blocks = (units + 15) / 16;
+    const int at = (int)blockIdx.x % blocks * 16 + (threadIdx.x >> 4);
+    KvUnit u;
+    u.head = at / (2 * c.nb);
+    u.is_v = at - u.head * 2 * c.nb >= c.nb;
+    u.b = at - u.head * 2 * c.nb - u.is_v * c.nb;
+    const int64_t quads = (tokens + 3) / 4;
+    const int shares = gridDim.x / blocks, share = blockIdx.x / blocks;
+    const int64_t each = (quads + shares - 1) / shares;
+    u.quad = each * share;
+    u.end = at < units ? (u.quad + each < quads ? u.quad + each : quads) : 0;
+    return u;
+}
+
+template <int DT, int RMODE, bool ZONE_ELEM>
 __global__ __launch_bounds__(TPB) void kv_append_kernel(KvRowsArgs a, MxParams p, uint32_t max_code) {
     constexpr int ADT = Arith<DT>::DT_;
     constexpr int ZS = (ADT == MXQ_BF16) ? 16 : 0;
     __shared__ unsigned char zone[ZONE_PAD];
     load_zone(zone, g_zone_tables[p.zone_row]);
     const int NB = a.c.nb, me = threadIdx.x & 3, j = (threadIdx.x >> 2) & 3;
-    const int64_t quads = (a.tokens + 3) / 4, per_quad = (int64_t)a.c.heads * NB * 2, items = quads * per_quad;
-    for (int64_t item = (int64_t)blockIdx.x * (TPB / 16) + (threadIdx.x >> 4); item < items; item += (int64_t)gridDim.x * (TPB / 16)) {
-        // items of a quad: head, then K or V, then block -- neighbouring lanes read neighbouring pieces of a row
-        const int64_t quad = item / per_quad;
-        const int rest = (int)(item - quad * per_quad);
-        const int head = rest / (2 * NB);
-        const int is_v = (rest - head * 2 * NB) >= NB, b = rest - head * 2 * NB - is_v * NB;
+    const KvUnit u = kv_unit(a.c, a.tokens);
+    const int head = u.head, is_v = u.is_v, b = u.b;
+    for (int64_t quad = u.quad; quad < u.end; ++quad) {
         const int64_t token = quad * 4 + me;
         const bool row = token < a.tokens;
         const int64_t slot = row ? a.slots[token] : -1;
@@ -236,12 +279,24 @@ __global__ __launch_bounds__(TPB) void kv_append_kernel(KvRowsArgs a, MxParams p
         const MxqScale sc = mxq_block_scale(um, p.emax, p.scale_emax, p.flush != 0, zone, ZS);
         const uint32_t sb = mxq_encode_e8m0(sc.scale);
         uint32_t codes = 0;
+        if constexpr (RMODE == MXQ_NEAREST && !ZONE_ELEM) {
+            using Nudge = KvNudge<ADT>;
+            const float inv = Nudge::inverse(sc.inv_scale);
+            float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            uint32_t c;
-            if constexpr (DIRECT) c = mxq_quant_mx_code<RMODE, ADT, 3>(x[e], sc, p.fmt, max_code);
-            else c = mxq_encode_e2m1(mxq_quant_mx_elem_unscaled<RMODE, ADT, ZONE_ELEM>(x[e], sc, p.fmt, zone, ZS));
-            codes |= c << (4 * e);
+            for (int e = 0; e < 8; ++e) y[e] = Nudge::apply(x[e], inv);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[0], y[1], 1.0f, 0);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[2], y[3], 1.0f, 1);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[4], y[5], 1.0f, 2);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[6], y[7], 1.0f, 3);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint32_t c;
+                if constexpr (!ZONE_ELEM) c = mxq_quant_mx_code<RMODE, ADT, 3>(x[e], sc, p.fmt, max_code);
+                else c = mxq_encode_e2m1(mxq_quant_mx_elem_unscaled<RMODE, ADT, ZONE_ELEM>(x[e], sc, p.fmt, zone, ZS));
+                codes |= c << (4 * e);
+            }
         }
         const KvPlace pl = kv_place(a.c, slot, head);
         const int ps = a.c.page_size;
@@ -267,6 +322,13 @@ __global__ __launch_bounds__(TPB) void kv_append_kernel(KvRowsArgs a, MxParams p
     }
 }
 
+template <int SEL>
+__device__ __forceinline__ void kv_decode_floats(uint32_t codes, float scale, float* y) {
+    const kv_f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, SEL);
+    y[2 * SEL] = v[0];
+    y[2 * SEL + 1] = v[1];
+}
+
 // The rows at `slots` as values: codes times scale, rounded once to the output type; rows without a slot are zero.
 struct KvReadArgs {
     void* k;
@@ -277,12 +339,14 @@ struct KvReadArgs {
 };
 template <int DT>
 __global__ __launch_bounds__(TPB) void kv_read_kernel(KvReadArgs a, int wide) {
+    // fp32 rows: a lane takes the elements 4 j .. and 16 + 4 j .. of the block instead of 8 j .., so that each of its two
+    // 16-byte stores lies next to its neighbours'
+    constexpr bool HALVES = DT == MXQ_F32;
     const int NB = a.c.nb, me = threadIdx.x & 3, j = (threadIdx.x >> 2) & 3;
-    const int64_t quads = (a.tokens + 3) / 4, per_quad = (int64_t)a.c.heads * NB * 2, items = quads * per_quad;
-    for (int64_t item = (int64_t)blockIdx.x * (TPB / 16) + (threadIdx.x >> 4); item < items; item += (int64_t)gridDim.x * (TPB / 16)) {
-        const int64_t quad = item / per_quad;
-        const int rest = (int)(item - quad * per_quad), head = rest / (2 * NB);
-        const int is_v = (rest - head * 2 * NB) >= NB, b = rest - head * 2 * NB - is_v * NB;
+    const auto pair = [&](int i) { return !HALVES ? 4 * j + i : i < 2 ? 2 * j + i : 6 + 2 * j + i; };   // of elements
+    const KvUnit u = kv_unit(a.c, a.tokens);
+    const int head = u.head, is_v = u.is_v, b = u.b;
+    for (int64_t quad = u.quad; quad < u.end; ++quad) {
         const int64_t token = quad * 4 + me;
         const int64_t slot = token < a.tokens ? a.slots[token] : -1;
         const KvPlace pl = kv_place(a.c, slot, head);
@@ -291,45 +355,52 @@ __global__ __launch_bounds__(TPB) void kv_read_kernel(KvReadArgs a, int wide) {
         uint32_t codes = 0, sb = 127;
         if (pl.live) {
             if (!is_v) {
-                codes = *reinterpret_cast<const uint32_t*>(pl.record + (int64_t)pl.off * (16 * NB) + 16 * b + 4 * j);
+                const unsigned char* kr = pl.record + (int64_t)pl.off * (16 * NB) + 16 * b;
+                if constexpr (HALVES)
+                    codes = *reinterpret_cast<const unsigned short*>(kr + 2 * j) |
+                            (uint32_t)*reinterpret_cast<const unsigned short*>(kr + 8 + 2 * j) << 16;
+                else codes = *reinterpret_cast<const uint32_t*>(kr + 4 * j);
                 sb = pl.record[(int64_t)ps * (32 * NB) + (int64_t)pl.off * NB + b];
             } else {
                 const unsigned char* vt = pl.record + (int64_t)ps * (16 * NB) + (int64_t)(pl.off >> 2) * (64 * NB) + 4 * b;
                 sb = pl.record[(int64_t)ps * (33 * NB) + (int64_t)(pl.off >> 2) * (4 * NB) + 4 * b + (pl.off & 3)];
                 if (tile) {
-                    codes = *reinterpret_cast<const uint32_t*>(vt + (4 * j + me) * 4 * NB);
+                    codes = *reinterpret_cast<const uint32_t*>(vt + pair(me) * 4 * NB);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) codes |= (uint32_t)vt[(4 * j + i) * 4 * NB + (pl.off & 3)] << (8 * i);
+                    for (int i = 0; i < 4; ++i) codes |= (uint32_t)vt[pair(i) * 4 * NB + (pl.off & 3)] << (8 * i);
                 }
             }
         }
         const uint32_t turned = quad_transpose(codes, me);
         if (is_v && tile) codes = turned;
-        const int e0 = 32 * b + 8 * j;
+        const int e0 = 32 * b + (HALVES ? 4 * j : 8 * j);
         if (token >= a.tokens || e0 >= a.c.head_dim) continue;
-        const float scale = sb == 255u ? mxq_float(MXQ_QNAN_BITS) : ldexpf(1.0f, (int)sb - 127);
         float y[8];
+        const float scale = mxq_float(sb << 23);         // (the exponent field counts: 255 is NaN, 0 is 2^-127)
+        kv_decode_floats<0>(codes, scale, y);
+        kv_decode_floats<1>(codes, scale, y);
+        kv_decode_floats<2>(codes, scale, y);
+        kv_decode_floats<3>(codes, scale, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float v = mxq_decode_e2m1((codes >> (4 * e)) & 15u) * scale;
-            y[e] = pl.live ? mxq_round_dt<Arith<DT>::DT_>(v) : 0.0f;
-        }
+        for (int e = 0; e < 8; ++e) y[e] = pl.live ? mxq_round_dt<Arith<DT>::DT_>(y[e]) : 0.0f;
         const int64_t at = (token * a.c.heads + head) * (int64_t)a.c.head_dim + e0;
         void* dst = is_v ? a.v : a.k;
         if (wide) {
             if constexpr (DT == MXQ_F32) {
                 u32x4* o = reinterpret_cast<u32x4*>(reinterpret_cast<float*>(dst) + at);
                 o[0] = u32x4{mxq_bits(y[0]), mxq_bits(y[1]), mxq_bits(y[2]), mxq_bits(y[3])};
-                o[1] = u32x4{mxq_bits(y[4]), mxq_bits(y[5]), mxq_bits(y[6]), mxq_bits(y[7])};
+                if (e0 + 16 < a.c.head_dim) o[4] = u32x4{mxq_bits(y[4]), mxq_bits(y[5]), mxq_bits(y[6]), mxq_bits(y[7])};
             } else {
                 *reinterpret_cast<u32x4*>(reinterpret_cast<unsigned short*>(dst) + at) =
                     u32x4{Pack<DT>::put(y[0], y[1]), Pack<DT>::put(y[2], y[3]), Pack<DT>::put(y[4], y[5]), Pack<DT>::put(y[6], y[7])};
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e0 + e < a.c.head_dim) store_scalar<DT>(dst, at + e, y[e]);
+            for (int e = 0; e < 8; ++e) {
+                const int d = HALVES && e >= 4 ? e + 12 : e;
+                if (e0 + d < a.c.head_dim) store_scalar<DT>(dst, at + d, y[e]);
+            }
         }
     }
 }

@@ -19,6 +19,7 @@ from .custom_extensions import _DTYPE, _flags_value, _stream
 from .formats import RoundingMode
 
 MAX_HEAD_DIM = 256
+_ROUNDINGS = {name: int(RoundingMode[name]) for name in RoundingMode.string_enums()}
 _TOKEN_BYTES = 34                 # K and V of a token, for each block of 32: 2 x (16 bytes of codes + 1 scale)
 
 
@@ -78,8 +79,21 @@ def _check_cache(cache, who):
 def _check_on(t, first, name, who):
     if not t.is_cuda:
         raise RuntimeError("%s: %s must be a CUDA tensor" % (who, name))
-    if t.device != first.device:
+    if t.get_device() != first.get_device():
         raise RuntimeError("%s: %s is on %s, not on %s" % (who, name, t.device, first.device))
+
+
+def _call(t, fn, *args):
+    """fn(*args, current stream) on t's device.  Where that is the current one already, as it nearly always is, the
+    context of torch.cuda.device and the stream object (3.5 us of a call of 10) are not needed."""
+    index = t.get_device()
+    if index >= 0 and index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(t.device):
+            rc = fn(*args, _stream(t))
+    if rc != 0:
+        _lib.check(rc, _lib.gpu())
 
 
 def _check_index(t, shape, dtype, first, name, who):
@@ -137,19 +151,15 @@ def kv_block_tables(context_lens, new_lens, block_table, free_pages, free_start,
     _check_index(new_lens, (R,), torch.int32, block_table, "new_lens", who)
     _check_index(free_pages, (None,), torch.int32, block_table, "free_pages", who)
     _check_index(free_start, (1,), torch.int32, block_table, "free_start", who)
-    device = block_table.device
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=device)
+    slots = block_table.new_empty(num_tokens, dtype=torch.int64)
     # the int32 results share one allocation
-    ints = torch.empty(2 * num_tokens + 2 * R + 2, dtype=torch.int32, device=device)
-    positions, requests, starts, seq_lens, free_next = ints.split([num_tokens, num_tokens, R + 1, R, 1])
-    lib = _lib.gpu()
-    with torch.cuda.device(device):
-        rc = lib.mxq_kv_block_tables(context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-                                     block_table.stride(0), block_table.shape[1], free_pages.data_ptr(), free_pages.numel(),
-                                     free_start.data_ptr(), R, page_size, num_tokens, slots.data_ptr(),
-                                     positions.data_ptr(), requests.data_ptr(), starts.data_ptr(), seq_lens.data_ptr(),
-                                     free_next.data_ptr(), _stream(block_table))
-    _lib.check(rc, lib)
+    ints = block_table.new_empty(2 * num_tokens + 2 * R + 2)
+    positions, requests, starts, seq_lens, free_next = ints.split_with_sizes((num_tokens, num_tokens, R + 1, R, 1))
+    at = ints.data_ptr()
+    _call(block_table, _lib.gpu().mxq_kv_block_tables, context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+          block_table.stride(0), block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_start.data_ptr(), R,
+          page_size, num_tokens, slots.data_ptr(), at, at + 4 * num_tokens, at + 8 * num_tokens,
+          at + 8 * num_tokens + 4 * (R + 1), at + 8 * num_tokens + 4 * (2 * R + 1))
     return KVBlockTables(block_table, slots, positions, requests, starts, seq_lens, free_next)
 
 
@@ -171,16 +181,13 @@ def kv_append(cache, k, v, slots, scale_bits=8, round="nearest", flush_fp32_subn
     if k.shape[0] != v.shape[0]:
         raise RuntimeError("%s: k has %d rows, v has %d" % (who, k.shape[0], v.shape[0]))
     _check_index(slots, (k.shape[0],), torch.int64, data, "slots", who)
-    if round not in RoundingMode.string_enums():
+    if round not in _ROUNDINGS:
         raise RuntimeError("%s: unknown rounding %r" % (who, round))
     _check_no_grad(who, k, v)
-    lib = _lib.gpu()
-    with torch.cuda.device(data.device):
-        rc = lib.mxq_kv_append_mx(k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], k.shape[0], k.stride(0), k.stride(1),
-                                  v.stride(0), v.stride(1), slots.data_ptr(), data.data_ptr(), data.shape[0], data.shape[1],
-                                  page_size, head_dim, scale_bits, int(bool(flush_fp32_subnorms)), int(RoundingMode[round]),
-                                  _flags_value(), _stream(data))
-    _lib.check(rc, lib)
+    ks, vs = k.stride(), v.stride()
+    _call(data, _lib.gpu().mxq_kv_append_mx, k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], k.shape[0], ks[0], ks[1], vs[0], vs[1],
+          slots.data_ptr(), data.data_ptr(), data.shape[0], data.shape[1], page_size, head_dim, scale_bits,
+          1 if flush_fp32_subnorms else 0, _ROUNDINGS[round], _flags_value())
 
 
 def kv_read(cache, slots, dtype=torch.float32):
@@ -193,12 +200,9 @@ def kv_read(cache, slots, dtype=torch.float32):
     if dtype not in _DTYPE:
         raise RuntimeError("%s: Tensor dtype not supported (%s)" % (who, dtype))
     shape = (slots.shape[0], data.shape[1], head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=data.device) for _ in range(2))
-    lib = _lib.gpu()
-    with torch.cuda.device(data.device):
-        rc = lib.mxq_kv_read_mx(k.data_ptr(), v.data_ptr(), _DTYPE[dtype], shape[0], slots.data_ptr(), data.data_ptr(),
-                                data.shape[0], data.shape[1], page_size, head_dim, _stream(data))
-    _lib.check(rc, lib)
+    k, v = data.new_empty(shape, dtype=dtype), data.new_empty(shape, dtype=dtype)
+    _call(data, _lib.gpu().mxq_kv_read_mx, k.data_ptr(), v.data_ptr(), _DTYPE[dtype], shape[0], slots.data_ptr(), data.data_ptr(),
+          data.shape[0], data.shape[1], page_size, head_dim)
     return k, v
 
 
@@ -235,12 +239,11 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
         raise RuntimeError("%s: without starts every request has one row: %d rows, %d requests" % (who, q.shape[0], R))
     if q.shape[0] * q.shape[1] > 0x7FFFFF00:
         raise RuntimeError("%s: q has too many rows" % who)
-    if scale is None:
-        scale = head_dim ** -0.5
+    scale = head_dim ** -0.5 if scale is None else float(scale)
     _check_no_grad(who, q)
     new = out is None
     if new:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     else:
         _check_rows(out, "out", who)
         _check_on(out, data, "out", who)
@@ -248,18 +251,15 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
             raise RuntimeError("%s: out must be %s %s, got %s %s" % (who, q.dtype, tuple(q.shape), out.dtype, tuple(out.shape)))
         if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
             raise RuntimeError("%s: rows of out share memory" % who)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    max_new = (1 if starts is None else q.shape[0]) if max_new is None else max(1, int(max_new))
-    lib = _lib.gpu()
     rows, q_heads, width = q.shape[0], q.shape[1], block_table.shape[1]
-    with torch.cuda.device(data.device):
-        ws_bytes = lib.mxq_kv_attention_workspace_bytes(R, rows, q_heads, max_new, width, heads, page_size, head_dim)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=data.device) if ws_bytes else None
-        rc = lib.mxq_kv_attention_mx(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                     None if lse is None else lse.data_ptr(), _DTYPE[q.dtype], rows, q_heads,
-                                     block_table.data_ptr(), block_table.stride(0), width, seq_lens.data_ptr(),
-                                     None if starts is None else starts.data_ptr(), R, float(scale), int(bool(causal)),
-                                     max_new, int(new), data.data_ptr(), data.shape[0], heads, page_size, head_dim,
-                                     None if ws is None else ws.data_ptr(), ws_bytes, _stream(data))
-    _lib.check(rc, lib)
+    lse = q.new_empty((rows, q_heads), dtype=torch.float32) if return_lse else None
+    max_new = (1 if starts is None else rows) if max_new is None else max(1, int(max_new))
+    lib, dtype, qs, outs = _lib.gpu(), _DTYPE[q.dtype], q.stride(), out.stride()
+    ws_bytes = lib.mxq_kv_attention_workspace_bytes(R, rows, q_heads, max_new, width, heads, page_size, head_dim, dtype)
+    ws = data.new_empty(ws_bytes) if ws_bytes else None
+    _call(data, lib.mxq_kv_attention_mx, q.data_ptr(), qs[0], qs[1], out.data_ptr(), outs[0], outs[1],
+          None if lse is None else lse.data_ptr(), dtype, rows, q_heads, block_table.data_ptr(), block_table.stride(0), width,
+          seq_lens.data_ptr(), None if starts is None else starts.data_ptr(), R, scale, 1 if causal else 0, max_new,
+          1 if new else 0, data.data_ptr(), data.shape[0], heads, page_size, head_dim, None if ws is None else ws.data_ptr(),
+          ws_bytes)
     return (out, lse) if return_lse else out

@@ -351,6 +351,18 @@ inline int __all(int pred) {                               // over the lanes of 
     return all;
 }
 
+inline uint64_t __ballot(int pred) {                       // one bit for each lane that is still there
+    emu::Block& b = *emu::block();
+    const int lane = emu::lane_in_block(), w = lane / emu::kWave;
+    b.slot[lane] = pred ? 1 : 0;
+    emu::wave_meet();
+    uint64_t bits = 0;
+    for (int l = 0; l < emu::kWave; ++l)
+        if (b.active[w * emu::kWave + l].load() && b.slot[w * emu::kWave + l] != 0) bits |= (uint64_t)1 << l;
+    emu::wave_meet();
+    return bits;
+}
+
 // v_readfirstlane_b32: the value of the first lane of the wave that is still there
 inline int emu_readfirstlane(int v) {
     emu::Block& b = *emu::block();
@@ -421,6 +433,22 @@ inline unsigned emu_perm(unsigned a, unsigned b, unsigned sel) {
 }
 #define __builtin_amdgcn_perm emu_perm
 
+// buffer loads: the address, the lane's offset and the uniform offset added up (no range is checked: none is given)
+typedef const unsigned char* __amdgpu_buffer_rsrc_t;
+typedef uint32_t emu_u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t emu_u32x4 __attribute__((ext_vector_type(4)));
+template <class T>
+inline T emu_buffer_load(const unsigned char* base, int lane_offset, int offset) {
+    T v;
+    memcpy(&v, base + (uint32_t)lane_offset + (uint64_t)(uint32_t)offset, sizeof(T));
+    return v;
+}
+#define __builtin_amdgcn_make_buffer_rsrc(p, stride, range, flags) (static_cast<const unsigned char*>(p))
+#define __builtin_amdgcn_raw_buffer_load_b8(r, v, s, aux) emu_buffer_load<uint8_t>(r, v, s)
+#define __builtin_amdgcn_raw_buffer_load_b32(r, v, s, aux) emu_buffer_load<uint32_t>(r, v, s)
+#define __builtin_amdgcn_raw_buffer_load_b64(r, v, s, aux) emu_buffer_load<emu_u32x2>(r, v, s)
+#define __builtin_amdgcn_raw_buffer_load_b128(r, v, s, aux) emu_buffer_load<emu_u32x4>(r, v, s)
+
 // v_log_f32 (base 2)
 #define __builtin_amdgcn_logf log2f
 
@@ -440,6 +468,35 @@ inline emu_bf16x2 emu_cvt_fp4(unsigned codes, float scale, int sel) {
     return __builtin_bit_cast(emu_bf16x2, out);
 }
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4 emu_cvt_fp4
+
+// v_cvt_scalef32_pk_f32_fp4, the same as fp32
+typedef float emu_f32x2 __attribute__((ext_vector_type(2)));
+inline emu_f32x2 emu_cvt_fp4_f32(unsigned codes, float scale, int sel) {
+    static const float mag[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
+    const int e = (int)((__float_as_uint(scale) >> 23) & 255u);
+    emu_f32x2 out;
+    for (int n = 0; n < 2; ++n) {
+        const unsigned c = (codes >> (8 * sel + 4 * n)) & 15u;
+        out[n] = e == 255 ? NAN : ldexpf((c & 8) ? -mag[c & 7] : mag[c & 7], e - 127);
+    }
+    return out;
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_f32_fp4 emu_cvt_fp4_f32
+
+// v_cvt_scalef32_pk_fp4_f32: two values over 2^(exponent field of scale - 127), rounded half to even, saturated at 6,
+// into byte `sel` of old
+inline unsigned emu_to_fp4(float x, int e) {
+    static const float mag[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
+    const float a = ldexpf(fabsf(x), 127 - e);
+    unsigned c = 0;
+    while (c < 7 && (a > (mag[c] + mag[c + 1]) / 2 || (a == (mag[c] + mag[c + 1]) / 2 && (c & 1)))) ++c;
+    return c | (signbit(x) ? 8u : 0u);
+}
+inline unsigned emu_cvt_f32_fp4(unsigned old, float a, float b, float scale, int sel) {
+    const int e = (int)((__float_as_uint(scale) >> 23) & 255u);
+    return (old & ~(255u << (8 * sel))) | ((emu_to_fp4(a, e) | emu_to_fp4(b, e) << 4) << (8 * sel));
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32 emu_cvt_f32_fp4
 
 // v_mfma_f32_16x16x32_bf16: lane l supplies row (column) l % 16, K = 8 (l / 16) .. + 7, and receives column l % 16,
 // rows 4 (l / 16) + r

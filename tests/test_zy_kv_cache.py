@@ -130,6 +130,34 @@ def test_special_values_and_fp16_rows():
     assert_bits_equal(got, want, "fp16, exact exponents")
 
 
+@pytest.mark.parametrize("round", ["nearest", "even", "floor"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_values_at_and_next_to_every_border(dtype, round):
+    """Every finite bf16 code beside block maxima that put it at every place of the grid (fp32: the borders between
+    codes and their neighbours), maxima at both ends of the range and in the zone where log2 rounds up."""
+    if dtype == torch.bfloat16:
+        codes = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16).float()
+        codes = codes[torch.isfinite(codes)]
+    else:
+        edges = torch.tensor([0, 0.25, 0.5, 0.75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 7, 2.0 ** -126, 2.0 ** -149, 1e-3])
+        bits = edges.view(torch.int32)[:, None] + torch.arange(-3, 4, dtype=torch.int32)
+        codes = bits.clamp(min=0).view(torch.float32).flatten()
+        codes = torch.cat([codes, -codes, codes * 2.0 ** -30, codes * 2.0 ** 20])
+    maxima = torch.tensor([4.0, 5.0, 6.5, 7.96875, 1.0, 2.0 ** -126, 2.0 ** -130, 3e38, 2.0 ** 127, 0.0078125]).to(dtype).float()
+    x = torch.zeros(len(maxima) * -(-len(codes) // 31), 1, 32)
+    n = -(-len(codes) // 31)
+    padded = torch.cat([codes, codes.new_zeros(n * 31 - len(codes))]).view(n, 31)
+    for i, m in enumerate(maxima):
+        part = x[i * n:(i + 1) * n, 0]
+        part[:, 0], part[:, 1:] = m, torch.where(padded.abs() <= m, padded, torch.zeros(()))
+    x = x.to(dtype)
+    cache = new_kv_cache(-(-len(x) // 16), 16, 1, 32, DEV)
+    slots = torch.arange(len(x), device=DEV)
+    kv_append(cache, x.to(DEV), (-x).to(DEV), slots, round=round)
+    for got, y in zip(kv_read(cache, slots), (x, -x)):
+        assert_bits_equal(got.cpu(), quantized(y, round), "codes")
+
+
 # ---- block tables ----------------------------------------------------------------------------------------------------
 def tables_by_loops(ctx, new, table, free, start, page, rows):
     table, R, C = [list(r) for r in table], len(ctx), len(table[0]) if table else 0
