@@ -83,12 +83,15 @@ def _check_on(t, first, name, who):
         raise RuntimeError("%s: %s is on %s, not on %s" % (who, name, t.device, first.device))
 
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _call(t, fn, *args):
     """fn(*args, current stream) on t's device.  Where that is the current one already, as it nearly always is, the
     context of torch.cuda.device and the stream object (3.5 us of a call of 10) are not needed."""
     index = t.get_device()
-    if index >= 0 and index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index >= 0 and index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(t.device):
             rc = fn(*args, _stream(t))
@@ -130,16 +133,7 @@ def _check_no_grad(who, *tensors):
         raise RuntimeError("%s: has no gradient (the cache holds rounded values): call it under torch.no_grad()" % who)
 
 
-def kv_block_tables(context_lens, new_lens, block_table, free_pages, free_start, page_size, num_tokens):
-    """Pages, slots and positions of a step's new tokens, from the requests' lengths (KVBlockTables).
-
-    Request r has context_lens[r] tokens in the pages of row r of block_table and gets new_lens[r] more (int32,
-    negative counts as zero).  The pages it lacks are taken from free_pages (int32) at free_start[0] on (int32, one
-    element), in the order of the requests, and entered into block_table in place.  num_tokens is the number of rows
-    that the step's tensors have: at least the sum of new_lens, rows behind it are marked -1, so that a padded batch
-    keeps its shapes.  Where the free pages or the row of the table end, tokens have slot -1: kv_append leaves them
-    out, kv_attention does not see them.  Repeating a call gives the same results; the returned free_start is what the
-    next step passes.  (Pages of a finished request go back to the list with free_pages[...] = block_table[r, :n].)"""
+def _check_block_tables(context_lens, new_lens, block_table, free_pages, free_start, page_size, num_tokens):
     who = "kv_block_tables"
     if page_size < 16 or page_size % 16 != 0 or page_size > 65536:
         raise RuntimeError("%s: page_size must be a multiple of 16 up to 65536, got %d" % (who, page_size))
@@ -151,26 +145,43 @@ def kv_block_tables(context_lens, new_lens, block_table, free_pages, free_start,
     _check_index(new_lens, (R,), torch.int32, block_table, "new_lens", who)
     _check_index(free_pages, (None,), torch.int32, block_table, "free_pages", who)
     _check_index(free_start, (1,), torch.int32, block_table, "free_start", who)
+
+
+def kv_block_tables(context_lens, new_lens, block_table, free_pages, free_start, page_size, num_tokens):
+    """Pages, slots and positions of a step's new tokens, from the requests' lengths (KVBlockTables).
+
+    Request r has context_lens[r] tokens in the pages of row r of block_table and gets new_lens[r] more (int32,
+    negative counts as zero).  The pages it lacks are taken from free_pages (int32) at free_start[0] on (int32, one
+    element), in the order of the requests, and entered into block_table in place.  num_tokens is the number of rows
+    that the step's tensors have: at least the sum of new_lens, rows behind it are marked -1, so that a padded batch
+    keeps its shapes.  Where the free pages or the row of the table end, tokens have slot -1: kv_append leaves them
+    out, kv_attention does not see them.  Repeating a call gives the same results; the returned free_start is what the
+    next step passes.  (Pages of a finished request go back to the list with free_pages[...] = block_table[r, :n].)"""
+    table, R, int32 = block_table.shape, context_lens.numel(), torch.int32
+    at = block_table.get_device()
+    if not (len(table) == 2 and table[0] == R and context_lens.shape == new_lens.shape == table[:1] and free_start.shape == (1,) and
+            free_pages.dim() == 1 and block_table.dtype is int32 and context_lens.dtype is int32 and new_lens.dtype is int32 and
+            free_pages.dtype is int32 and free_start.dtype is int32 and block_table.is_cuda and
+            at == context_lens.get_device() == new_lens.get_device() == free_pages.get_device() == free_start.get_device() and
+            block_table.is_contiguous() and context_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous() and
+            page_size % 16 == 0 and 16 <= page_size <= 65536 and 0 <= num_tokens <= 0x7FFFFF00 and table[1] * page_size <= 1 << 30):
+        _check_block_tables(context_lens, new_lens, block_table, free_pages, free_start, page_size, num_tokens)
     slots = block_table.new_empty(num_tokens, dtype=torch.int64)
     # the int32 results share one allocation
     ints = block_table.new_empty(2 * num_tokens + 2 * R + 2)
     positions, requests, starts, seq_lens, free_next = ints.split_with_sizes((num_tokens, num_tokens, R + 1, R, 1))
-    at = ints.data_ptr()
+    first = ints.data_ptr()
     _call(block_table, _lib.gpu().mxq_kv_block_tables, context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-          block_table.stride(0), block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_start.data_ptr(), R,
-          page_size, num_tokens, slots.data_ptr(), at, at + 4 * num_tokens, at + 8 * num_tokens,
-          at + 8 * num_tokens + 4 * (R + 1), at + 8 * num_tokens + 4 * (2 * R + 1))
+          block_table.stride(0), table[1], free_pages.data_ptr(), free_pages.numel(), free_start.data_ptr(), R,
+          page_size, num_tokens, slots.data_ptr(), first, first + 4 * num_tokens, first + 8 * num_tokens,
+          first + 8 * num_tokens + 4 * (R + 1), first + 8 * num_tokens + 4 * (2 * R + 1))
     return KVBlockTables(block_table, slots, positions, requests, starts, seq_lens, free_next)
 
 
-def kv_append(cache, k, v, slots, scale_bits=8, round="nearest", flush_fp32_subnorms=False):
-    """Quantizes rows k, v (rows, heads, head_dim; any strides with contiguous elements) as pack_mx does and stores them
-    at `slots` (int64, one a row) of the cache, in place.  Rows whose slot is negative or beyond the cache are left out.
-    No slot may be named twice in a call: which row it would then hold is not defined.  fp16 rows need
-    custom_extensions.set_exponent_mode('exact'), as for pack_mx."""
+def _check_append(cache, k, v, slots, round):
     who = "kv_append"
     _check_cache(cache, who)
-    data, page_size, head_dim = cache
+    data, _, head_dim = cache
     for t, name in ((k, "k"), (v, "v")):
         _check_rows(t, name, who)
         _check_on(t, data, name, who)
@@ -184,42 +195,51 @@ def kv_append(cache, k, v, slots, scale_bits=8, round="nearest", flush_fp32_subn
     if round not in _ROUNDINGS:
         raise RuntimeError("%s: unknown rounding %r" % (who, round))
     _check_no_grad(who, k, v)
-    ks, vs = k.stride(), v.stride()
-    _call(data, _lib.gpu().mxq_kv_append_mx, k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], k.shape[0], ks[0], ks[1], vs[0], vs[1],
-          slots.data_ptr(), data.data_ptr(), data.shape[0], data.shape[1], page_size, head_dim, scale_bits,
+
+
+def kv_append(cache, k, v, slots, scale_bits=8, round="nearest", flush_fp32_subnorms=False):
+    """Quantizes rows k, v (rows, heads, head_dim; any strides with contiguous elements) as pack_mx does and stores them
+    at `slots` (int64, one a row) of the cache, in place.  Rows whose slot is negative or beyond the cache are left out.
+    No slot may be named twice in a call: which row it would then hold is not defined.  fp16 rows need
+    custom_extensions.set_exponent_mode('exact'), as for pack_mx."""
+    who = "kv_append"
+    data, page_size, head_dim = cache
+    at, shape, rows, ks, vs = data.get_device(), data.shape, k.shape, k.stride(), v.stride()
+    # one look at what has to hold (2 us less of a call); what is wrong is named by the checks one by one
+    if not (len(shape) == 3 and len(rows) == 3 and rows == v.shape and rows[1] == shape[1] and rows[2] == head_dim and
+            shape[2] == _record_bytes(page_size, head_dim) and ks[2] == 1 and vs[2] == 1 and slots.shape == rows[:1] and
+            k.dtype in _DTYPE and v.dtype is k.dtype and data.dtype is torch.uint8 and slots.dtype is torch.int64 and
+            at == k.get_device() == v.get_device() == slots.get_device() and k.is_cuda and data.is_contiguous() and
+            slots.is_contiguous() and round in _ROUNDINGS and not (k.requires_grad or v.requires_grad) and
+            page_size % 16 == 0 and 16 <= page_size <= 65536 and 1 <= head_dim <= MAX_HEAD_DIM and shape[0] > 0 and shape[1] > 0):
+        _check_append(cache, k, v, slots, round)
+    _call(data, _lib.gpu().mxq_kv_append_mx, k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], rows[0], ks[0], ks[1], vs[0], vs[1],
+          slots.data_ptr(), data.data_ptr(), shape[0], shape[1], page_size, head_dim, scale_bits,
           1 if flush_fp32_subnorms else 0, _ROUNDINGS[round], _flags_value())
 
 
 def kv_read(cache, slots, dtype=torch.float32):
     """(k, v): the values stored at `slots` (int64), each (rows, heads, head_dim) of `dtype`; zeros for slots outside the
     cache.  A block that held Inf or NaN when it was stored is NaN, as with quantize_mx."""
-    who = "kv_read"
-    _check_cache(cache, who)
     data, page_size, head_dim = cache
-    _check_index(slots, (None,), torch.int64, data, "slots", who)
-    if dtype not in _DTYPE:
-        raise RuntimeError("%s: Tensor dtype not supported (%s)" % (who, dtype))
-    shape = (slots.shape[0], data.shape[1], head_dim)
+    sizes, n = data.shape, slots.shape
+    if not (len(sizes) == 3 and len(n) == 1 and sizes[2] == _record_bytes(page_size, head_dim) and dtype in _DTYPE and
+            data.dtype is torch.uint8 and slots.dtype is torch.int64 and data.get_device() == slots.get_device() and data.is_cuda and
+            data.is_contiguous() and slots.is_contiguous() and page_size % 16 == 0 and 16 <= page_size <= 65536 and
+            1 <= head_dim <= MAX_HEAD_DIM and sizes[0] > 0 and sizes[1] > 0):
+        who = "kv_read"
+        _check_cache(cache, who)
+        _check_index(slots, (None,), torch.int64, data, "slots", who)
+        if dtype not in _DTYPE:
+            raise RuntimeError("%s: Tensor dtype not supported (%s)" % (who, dtype))
+    shape = (n[0], sizes[1], head_dim)
     k, v = data.new_empty(shape, dtype=dtype), data.new_empty(shape, dtype=dtype)
     _call(data, _lib.gpu().mxq_kv_read_mx, k.data_ptr(), v.data_ptr(), _DTYPE[dtype], shape[0], slots.data_ptr(), data.data_ptr(),
-          data.shape[0], data.shape[1], page_size, head_dim)
+          sizes[0], sizes[1], page_size, head_dim)
     return k, v
 
 
-def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causal=True, max_new=None, out=None,
-                 return_lse=False):
-    """softmax(scale * q K^T) V over the cached tokens of each row's request; q (rows, query heads, head_dim), bf16 or
-    fp16, any strides with contiguous elements.  Query head h reads kv head h // (query heads // kv heads).
-
-    seq_lens (int32): tokens of each request, the new ones (already appended) included.  starts (int32, requests + 1):
-    request r has the rows starts[r] .. starts[r + 1] - 1, which are its last tokens; None: one row a request.  With
-    causal a row sees the tokens up to its own, otherwise all of its request.  Tokens whose page is not in the cache are
-    not seen.  A row that sees no token gets zeros (lse -inf).  Rows behind the last request are zero (lse -inf) in a new
-    output and left as they are in a given `out`.  scale defaults to head_dim ** -0.5.
-
-    max_new: the most rows that a request has, if known: it steers the choice of kernels, never the result.  return_lse:
-    also the logarithm of the sum of exponentials, fp32 (rows, query heads).  Accumulation, maxima and sums are fp32; the
-    probabilities enter the second product as bf16 (two bf16 terms for few rows a request and for fp16 queries)."""
+def _check_attention(q, cache, block_table, seq_lens, starts, out):
     who = "kv_attention"
     _check_cache(cache, who)
     data, page_size, head_dim = cache
@@ -239,27 +259,57 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
         raise RuntimeError("%s: without starts every request has one row: %d rows, %d requests" % (who, q.shape[0], R))
     if q.shape[0] * q.shape[1] > 0x7FFFFF00:
         raise RuntimeError("%s: q has too many rows" % who)
-    scale = head_dim ** -0.5 if scale is None else float(scale)
     _check_no_grad(who, q)
-    new = out is None
-    if new:
-        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
-    else:
+    if out is not None:
         _check_rows(out, "out", who)
         _check_on(out, data, "out", who)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise RuntimeError("%s: out must be %s %s, got %s %s" % (who, q.dtype, tuple(q.shape), out.dtype, tuple(out.shape)))
         if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
             raise RuntimeError("%s: rows of out share memory" % who)
-    rows, q_heads, width = q.shape[0], q.shape[1], block_table.shape[1]
+
+
+def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causal=True, max_new=None, out=None,
+                 return_lse=False):
+    """softmax(scale * q K^T) V over the cached tokens of each row's request; q (rows, query heads, head_dim), bf16 or
+    fp16, any strides with contiguous elements.  Query head h reads kv head h // (query heads // kv heads).
+
+    seq_lens (int32): tokens of each request, the new ones (already appended) included.  starts (int32, requests + 1):
+    request r has the rows starts[r] .. starts[r + 1] - 1, which are its last tokens; None: one row a request.  With
+    causal a row sees the tokens up to its own, otherwise all of its request.  Tokens whose page is not in the cache are
+    not seen.  A row that sees no token gets zeros (lse -inf).  Rows behind the last request are zero (lse -inf) in a new
+    output and left as they are in a given `out`.  scale defaults to head_dim ** -0.5.
+
+    max_new: the most rows that a request has, if known: it steers the choice of kernels, never the result.  return_lse:
+    also the logarithm of the sum of exponentials, fp32 (rows, query heads).  Accumulation, maxima and sums are fp32; the
+    probabilities enter the second product as bf16 (two bf16 terms for few rows a request and for fp16 queries)."""
+    data, page_size, head_dim = cache
+    at, shape, table, q_shape, R = data.get_device(), data.shape, block_table.shape, q.shape, seq_lens.numel()
+    qs, heads = q.stride(), shape[1] if len(shape) == 3 else 0
+    # one look at what has to hold; what is wrong, or only unusual, is for the checks one by one
+    if not (out is None and len(q_shape) == 3 and len(table) == 2 and q_shape[2] == head_dim and qs[2] == 1 and
+            heads > 0 and shape[0] > 0 and q_shape[1] > 0 and q_shape[1] % heads == 0 and seq_lens.shape == table[:1] and
+            shape[2] == _record_bytes(page_size, head_dim) and (q.dtype is torch.bfloat16 or q.dtype is torch.float16) and
+            data.dtype is torch.uint8 and seq_lens.dtype is torch.int32 and block_table.dtype is torch.int32 and
+            (q_shape[0] == R if starts is None else starts.dtype is torch.int32 and starts.shape == (R + 1,) and
+             starts.get_device() == at and starts.is_contiguous()) and
+            at == q.get_device() == block_table.get_device() == seq_lens.get_device() and q.is_cuda and data.is_contiguous() and
+            block_table.is_contiguous() and seq_lens.is_contiguous() and not q.requires_grad and q_shape[0] * q_shape[1] < 1 << 30 and
+            page_size % 16 == 0 and 16 <= page_size <= 65536 and 1 <= head_dim <= MAX_HEAD_DIM and table[1] * page_size <= 1 << 30):
+        _check_attention(q, cache, block_table, seq_lens, starts, out)
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    new = out is None
+    if new:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q_shape)
+    rows, q_heads, width = q_shape[0], q_shape[1], table[1]
     lse = q.new_empty((rows, q_heads), dtype=torch.float32) if return_lse else None
     max_new = (1 if starts is None else rows) if max_new is None else max(1, int(max_new))
-    lib, dtype, qs, outs = _lib.gpu(), _DTYPE[q.dtype], q.stride(), out.stride()
+    lib, dtype, outs = _lib.gpu(), _DTYPE[q.dtype], out.stride()
     ws_bytes = lib.mxq_kv_attention_workspace_bytes(R, rows, q_heads, max_new, width, heads, page_size, head_dim, dtype)
     ws = data.new_empty(ws_bytes) if ws_bytes else None
     _call(data, lib.mxq_kv_attention_mx, q.data_ptr(), qs[0], qs[1], out.data_ptr(), outs[0], outs[1],
           None if lse is None else lse.data_ptr(), dtype, rows, q_heads, block_table.data_ptr(), block_table.stride(0), width,
           seq_lens.data_ptr(), None if starts is None else starts.data_ptr(), R, scale, 1 if causal else 0, max_new,
-          1 if new else 0, data.data_ptr(), data.shape[0], heads, page_size, head_dim, None if ws is None else ws.data_ptr(),
+          1 if new else 0, data.data_ptr(), shape[0], heads, page_size, head_dim, None if ws is None else ws.data_ptr(),
           ws_bytes)
     return (out, lse) if return_lse else out
