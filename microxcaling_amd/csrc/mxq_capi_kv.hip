@@ -68,13 +68,13 @@ Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64
     p.decode_columns = p.prompt ? 64 : 0x7FFFFFFF;
     p.ct = columns <= 16 ? 1 : kv_decode_most_ct(nb, terms);
     const int64_t units = ceil_div(room, KV_UNIT) > 0 ? ceil_div(room, KV_UNIT) : 1;
-    p.decode_items = rows * group / (16 * p.ct) + requests;
+    p.decode_items = rows * group / (16 * p.ct) + (requests > 0 ? requests : 1);
     p.whole = units <= 4;
     const int64_t chip = 256 * kv_decode_waves(nb, p.ct, terms);
     p.shares = ceil_div(chip, heads) < KV_MAX_SHARES ? ceil_div(chip, heads) : KV_MAX_SHARES;
     if (p.shares > p.decode_items * units) p.shares = p.decode_items * units;
     const int64_t cols = 64 * kv_prompt_ct(nb, terms);
-    p.prompt_items = rows * group / cols + requests;
+    p.prompt_items = rows * group / cols + (requests > 0 ? requests : 1);
     p.prompt_shares = 256 * (nb <= 4 ? 2 : 1) / heads > 1 ? 256 * (nb <= 4 ? 2 : 1) / heads : 1;
     return p;
 }
@@ -83,11 +83,12 @@ Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64
 int64_t decode_part_bytes(const Plan& p, int heads) {
     return p.whole ? 0 : p.shares * heads * 2 * (16 * p.ct) * (32 * p.nb + 2) * (int64_t)sizeof(float);
 }
+int64_t span_bytes(const Plan& p) { return p.whole ? 0 : ceil_div(p.decode_items, 2) * 16; }
 int64_t prompt_part_bytes(const Plan& p, int heads, int terms) {
     return p.prompt ? p.prompt_shares * heads * 2 * (64 * kv_prompt_ct(p.nb, terms)) * (32 * p.nb + 2) * (int64_t)sizeof(float) : 0;
 }
 int64_t part_bytes(const Plan& p, int heads, int terms, int64_t requests) {
-    return decode_part_bytes(p, heads) + prompt_part_bytes(p, heads, terms) +
+    return decode_part_bytes(p, heads) + span_bytes(p) + prompt_part_bytes(p, heads, terms) +
            (p.prompt ? kv_plan_bytes(p.prompt_items, p.prompt_shares, requests) : 0);
 }
 
@@ -226,7 +227,7 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     const Plan p = make_plan(requests, rows, q_heads / heads, max_new, width * page_size, heads, a.c.nb, terms);
     const int64_t needed = part_bytes(p, heads, terms, requests);
     // units and items are numbered in 32 bits
-    const int64_t most_units = (requests + ceil_div(rows * q_heads / heads, 16)) * (ceil_div(width * page_size, KV_UNIT) + 1);
+    const int64_t most_units = (requests + ceil_div(rows * q_heads / heads, 16)) * (ceil_div(width * page_size, KV_UNIT) + 1 + KV_ITEM_UNITS);
     // .. and so are the workgroups of a launch
     if (most_units > 0x7FFFFFFF || p.prompt_items * heads * 16 + (int64_t)64 * requests * heads > 0x7FFFFFFF || p.decode_items * heads > 0x7FFFFFFF) return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
     if (workspace_bytes < needed || (needed > 0 && !workspace))
@@ -254,7 +255,7 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.q_wide = aligned16(q) && head_dim % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     a.out_wide = aligned16(out) && head_dim % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0;
     a.zero_tail = zero_tail ? 1 : 0;
-    a.tile_columns = 16 * p.ct;
+    a.item_shift = p.ct == 1 ? 4 : 5;
     a.decode_columns = p.decode_columns;
     a.whole = p.whole ? 1 : 0;
     a.direct = p.whole && !starts && a.group <= 16 * p.ct ? 1 : 0;
@@ -262,6 +263,8 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.join_rows = p.prompt ? p.decode_columns / a.group : 0;
     a.part = reinterpret_cast<float*>(workspace);
     unsigned char* behind = reinterpret_cast<unsigned char*>(workspace) + decode_part_bytes(p, heads);
+    a.spans = reinterpret_cast<kv_i32x2*>(behind);
+    behind += span_bytes(p);
     a.prompt_part = p.prompt ? reinterpret_cast<float*>(behind) : nullptr;
     a.plan = p.prompt ? behind + prompt_part_bytes(p, heads, terms) : nullptr;
     a.prompt_shares = (int)p.prompt_shares;

@@ -25,6 +25,7 @@
 namespace {
 
 typedef float kv_f32x2 __attribute__((ext_vector_type(2)));
+typedef int kv_i32x2 __attribute__((ext_vector_type(2)));
 typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 kv_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 kv_bf16x2 __attribute__((ext_vector_type(2)));

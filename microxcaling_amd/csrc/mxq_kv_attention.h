@@ -36,12 +36,13 @@ struct KvAttnArgs {
     float scale_log2;                                    // |scale| log2(e)
     int negative;                                        // scale is
     int causal, q_wide, out_wide, zero_tail;
-    int tile_columns;                                    // decode: columns of an item, 16 CT
+    int item_shift;                                      // decode: an item has 2^item_shift = 16 CT columns
     int decode_columns;                                  // requests with more columns belong to the prompt kernel
     int whole;                                           // decode: a workgroup for each item, nothing to join
     int direct;                                          // .. and one item for each request
     int shares;                                          // decode: workgroups of a kv head, at most KV_MAX_SHARES
     int join_rows;                                       // join: so many rows of each request, or 0: every row
+    kv_i32x2* spans;                                     // decode: where the parts of each item lie (KvSpan)
     float* part;                                         // decode: partial results, two places for each workgroup
     int join_blocks;                                     // join: workgroups for decode rows, the others for prompt items
     int prompt_shares, prompt_items;                     // prompt: workgroups of a kv head and items of it, at most
@@ -87,18 +88,20 @@ __device__ __forceinline__ int kv_limit(const KvAttnArgs& a, const KvSeq& s, int
 constexpr float KV_NOTHING = -3.0e38f;
 constexpr int KV_MAX_SHARES = 1024;
 constexpr int KV_UNIT = 128;                             // tokens of a unit of work: a tile of 32 for each wave
+constexpr int KV_ITEM_UNITS = 3;                         // what beginning and ending an item counts for when work is dealt out
 
 // units and column groups of a request in the decode kernel; a request without keys still has one unit, whose
 // workgroup writes the zeros
 struct KvWork {
     int units, groups;
-    __device__ __forceinline__ int count() const { return units * groups; }  // (all of them together: below 2^31)
+    __device__ __forceinline__ int per() const { return units + KV_ITEM_UNITS; }
+    __device__ __forceinline__ int count() const { return per() * groups; }  // (all of them together: below 2^31)
 };
 __device__ __forceinline__ KvWork kv_work(const KvAttnArgs& a, const KvSeq& s) {
     const int columns = s.fresh * a.group;
     if (columns == 0 || columns > a.decode_columns) return KvWork{0, 0};
     const int units = (s.keys + KV_UNIT - 1) / KV_UNIT;
-    return KvWork{units > 0 ? units : 1, (columns + a.tile_columns - 1) / a.tile_columns};
+    return KvWork{units > 0 ? units : 1, (columns + (1 << a.item_shift) - 1) >> a.item_shift};
 }
 
 // ---- loads -------------------------------------------------------------------------------------------------------
@@ -224,6 +227,26 @@ struct KvKeys {                                          // what a lane holds of
 template <int NB>
 struct KvValues {                                        // .. and values
     uint32_t v[2][NB], vs[2][NB];
+};
+
+// Waves that share a SIMD take their turns by priority, then by age: left to age alone, the oldest workgroup of a compute
+// unit is done long before the youngest, which then has nobody to hide its waits behind.  So a wave lowers its priority
+// with every quarter of its work (64 requests with 1900 tokens on average, 8 x 4 heads of 128: 36.7 -> 34.6 us).
+struct KvPace {
+    int left, quarter;                                   // units of work, a tile of the wave each
+    __device__ __forceinline__ void at(int units_left) {
+        left = units_left;
+        if (left > 3 * quarter) __builtin_amdgcn_s_setprio(3);
+        else if (left > 2 * quarter) __builtin_amdgcn_s_setprio(2);
+        else if (left > quarter) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+    }
+    __device__ __forceinline__ void tile() {
+        --left;
+        if (left == 3 * quarter) __builtin_amdgcn_s_setprio(2);
+        else if (left == 2 * quarter) __builtin_amdgcn_s_setprio(1);
+        else if (left == quarter) __builtin_amdgcn_s_setprio(0);
+    }
 };
 
 // the columns of a wave
@@ -475,10 +498,9 @@ struct KvWave {
     }
 
     // The tiles first, first + stride, .. of 32 tokens below tile `end`.  The places of 32 tiles sit in the lanes (lane:
-    // tile lane / 2, half lane % 2).  DEPTH tiles are under way: a tile's keys are loaded as soon as those that lay in
-    // the same registers have been multiplied, its values likewise.
-    template <int DEPTH>
-    __device__ __forceinline__ void walk(const KvAttnArgs& a, int r, int head, int first, int end, int stride) {
+    // tile lane / 2, half lane % 2).  A tile's keys are loaded as soon as the last one's, in the same registers, have been
+    // multiplied, its values likewise.
+    __device__ __forceinline__ void walk(const KvAttnArgs& a, int r, int head, int first, int end, int stride, KvPace& pace) {
         const int seen_end = (max_limit + 31) / 32;      // uniform: nothing behind it is seen
         if (end > seen_end) end = seen_end;
         place(a);
@@ -488,25 +510,19 @@ struct KvWave {
             const uint64_t there = __ballot(p.there);
             int tiles = (end - chunk + stride - 1) / stride;
             if (tiles > 32) tiles = 32;
-            KvKeys<NB> keys[DEPTH];
-            KvValues<NB> values[DEPTH];
-            // no load is conditional: behind the last tile it is loaded again, and multiplied with nothing of it seen.
-            // The waits count the loads under way, and a branch around one would make them wait for more than needed.
+            KvKeys<NB> keys;
+            KvValues<NB> values;
+            // no load is conditional: behind the last tile it is loaded again.  The waits count the loads under way, and a
+            // branch around one would make them wait for more than needed.  They are issued in the loop's order, on which
+            // the waits rely.
             const int last = tiles - 1;
-#pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                // in the order of the loop's loads, on which its waits rely
-                fetch_keys(a, keys[d], p, d < last ? d : last);
-                __builtin_amdgcn_sched_barrier(0);
-                fetch_values(a, values[d], p, d < last ? d : last);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            for (int n0 = 0; n0 < tiles; n0 += DEPTH) {
-#pragma unroll
-                for (int d = 0; d < DEPTH; ++d) {
-                    const int n = n0 + d, after = n + DEPTH < last ? n + DEPTH : last;
-                    step(a, keys[d], values[d], p, n <= last ? (int)(there >> (2 * n)) & 3 : 0, after, 32 * (chunk + n * stride));
-                }
+            fetch_keys(a, keys, p, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_values(a, values, p, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            for (int n = 0; n < tiles; ++n) {
+                pace.tile();
+                step(a, keys, values, p, (int)(there >> (2 * n)) & 3, n < last ? n + 1 : last, 32 * (chunk + n * stride));
             }
         }
     }
@@ -574,13 +590,13 @@ __device__ __forceinline__ float kv_lse(float m, float l) {
 // where the partial results of a workgroup's first (0) or last (1) item lie, by column: elements, and behind all of
 // them maximum and sum
 __device__ __forceinline__ int64_t kv_part_row(const KvAttnArgs& a, int64_t share, int head, int place, int column) {
-    return ((share * a.c.heads + head) * 2 + place) * a.tile_columns + column;
+    return ((((share * a.c.heads + head) * 2 + place) << a.item_shift) + column);
 }
 template <int NB>
 __device__ __forceinline__ float* kv_part(const KvAttnArgs& a, int64_t row) { return a.part + row * (32 * NB); }
 template <int NB>
 __device__ __forceinline__ float* kv_part_ml(const KvAttnArgs& a, int64_t row) {
-    return a.part + (int64_t)a.shares * a.c.heads * 2 * a.tile_columns * (32 * NB) + 2 * row;
+    return a.part + ((int64_t)a.shares * a.c.heads * 2 << a.item_shift) * (32 * NB) + 2 * row;
 }
 
 template <int DT>
@@ -734,9 +750,13 @@ __device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* 
 
 // ---- few columns -----------------------------------------------------------------------------------------------
 // Units of all requests (each 128 tokens of one column group) are numbered through and dealt out to the workgroups of a
-// head in order, as evenly as it goes: the first `more` of them have one unit more than `each`.
+// head in order, as evenly as it goes: the first `more` of them have one number more than `each`.  Beginning and ending
+// an item (its q, the first loads, the sum over four waves) takes as long as some units, so every item has KV_ITEM_UNITS
+// numbers before its units: without them a workgroup with four short requests ended long after the others (64 requests of
+// 128 to 8192 tokens: 39.1 us; with 2, 3, 4 of them 34.3, 34.6, 35.7; 32 requests of 32 to 2048: 16.0 and 14.2, 13.7, 13.8).
 struct KvShares {
-    int each, more;
+    int each = 0, more = 0;
+    KvShares() = default;
     __device__ __forceinline__ KvShares(int units, int shares) : each(units / shares), more(units - units / shares * shares) {}
     __device__ __forceinline__ int begin(int w) const { return w * each + (w < more ? w : more); }
     __device__ __forceinline__ int of(int unit) const {
@@ -745,14 +765,15 @@ struct KvShares {
     }
 };
 
-// Registers of a wave: accumulators, q, the tiles under way and the rest; the waves that share a SIMD and the tiles
-// that each has under way follow from them.
-constexpr int kv_decode_registers(int nb, int ct, int terms, int depth) {
-    return nb * (8 * ct + 4 * ct * terms + 7 * depth) + 80 + 18 * ct - 8 + 10 * (terms - 1);
-}
-constexpr int kv_decode_depth(int, int, int) { return 1; }
+// The first item (16 CT columns of a request) of request r, in an order that needs no sums over requests: every item has a
+// number of its own, below rows G / (16 CT) + requests.
+__device__ __forceinline__ int kv_item(const KvAttnArgs& a, const KvSeq& s, int r) { return ((s.row0 * a.group) >> a.item_shift) + r; }
+
+// Waves that share a SIMD, from the registers of a wave: accumulators, q, the tile under way and the rest.
+constexpr int kv_decode_registers(int nb, int ct, int terms) { return nb * (8 * ct + 4 * ct * terms + 7) + 72 + 18 * ct + 10 * (terms - 1); }
 constexpr int kv_decode_waves(int nb, int ct, int terms) {
-    return kv_decode_registers(nb, ct, terms, 1) <= 126 ? 4 : kv_decode_registers(nb, ct, terms, 1) <= 168 ? 3 : kv_decode_registers(nb, ct, terms, 1) <= 245 && nb != 7 && (nb != 6 || terms == 1) ? 2 : 1;
+    const int n = kv_decode_registers(nb, ct, terms);
+    return n <= 126 ? 4 : n <= 168 ? 3 : n <= 245 && nb != 7 && (nb != 6 || terms == 1) ? 2 : 1;
 }
 // two tiles of columns for one reading of the tokens, where the registers allow it
 constexpr int kv_decode_most_ct(int nb, int terms) { return nb * (23 + 8 * terms) + 100 <= 240 ? 2 : 1; }
@@ -785,21 +806,48 @@ void kv_decode_kernel(KvAttnArgs a) {
     }
 
     // the workgroup's numbers at .. end - 1: units, or with a workgroup for each item (whole) items
-    int at = share, end = share + 1, window = share, number = share;
-    if (!a.direct) {                                     // (direct: one item a request, a workgroup for each)
-        const auto count_of = [&](int r) {
-            if (r >= a.requests) return 0;
-            const KvWork w = kv_work(a, kv_seq(a, r));
-            return a.whole ? w.groups : w.count();
-        };
-        int mine = count_of(threadIdx.x), sum, upto = block_scan(mine, s_wave, &sum), total = sum;
+    int at = share, end = share + 1, window = share, number = share, k0 = 0;
+    // 64 requests at a time sit in the lanes
+    const int lane = threadIdx.x & 63;
+    KvSeq in_lane{0, 0, 0, 0};
+    KvWork work_in_lane{0, 0};
+    const auto look = [&](int r) {
+        in_lane = KvSeq{0, 0, 0, 0};
+        work_in_lane = KvWork{0, 0};
+        if (r < a.requests) {
+            in_lane = kv_seq(a, r);
+            work_in_lane = kv_work(a, in_lane);
+        }
+        return a.whole ? work_in_lane.groups : work_in_lane.count();
+    };
+    const bool few = a.requests <= 64;
+    KvShares deal;
+    if (!a.direct && few) {                              // every wave finds its place by itself
+        const int mine = look(lane);
+        int upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += o;
+        }
+        const int total = __builtin_amdgcn_readlane(upto, 63);
+        if (!a.whole) {
+            deal = KvShares(total, a.shares);
+            at = deal.begin(share);
+            end = deal.begin(share + 1);
+        }
+        if (at >= end || at >= total) return;
+        k0 = uniform(__builtin_ctzll(__ballot(at < upto)));                  // the first request that ends behind `at`
+        number = __builtin_amdgcn_readlane(upto - mine, k0);
+        window = 0;
+    } else if (!a.direct) {                              // (direct: one item a request, a workgroup for each)
+        int mine = look(threadIdx.x), sum, upto = block_scan(mine, s_wave, &sum), total = sum;
         if (a.requests > TPB) {
             int rest = 0;
-            for (int r = TPB + threadIdx.x; r < a.requests; r += TPB) rest += count_of(r);
+            for (int r = TPB + threadIdx.x; r < a.requests; r += TPB) rest += look(r);
             total += block_sum(rest, s_wave);
         }
         if (!a.whole) {
-            const KvShares deal(total, a.shares);
+            deal = KvShares(total, a.shares);
             at = deal.begin(share);
             end = deal.begin(share + 1);
         }
@@ -813,7 +861,7 @@ void kv_decode_kernel(KvAttnArgs a) {
             }
             before += sum;
             if (at < before) break;
-            mine = count_of(r0 + TPB + threadIdx.x);
+            mine = look(r0 + TPB + threadIdx.x);
             upto = block_scan(mine, s_wave, &sum);
         }
         __syncthreads();
@@ -821,33 +869,34 @@ void kv_decode_kernel(KvAttnArgs a) {
         number = uniform(s_found[1]);
     }
     const int first_number = at;
-    // 64 requests at a time sit in the lanes
-    const int lane = threadIdx.x & 63;
-    for (; at < end && window < a.requests; window += 64) {
-        KvSeq in_lane{0, 0, 0, 0};
-        KvWork work_in_lane{0, 0};
-        if (window + lane < a.requests) {
-            in_lane = kv_seq(a, window + lane);
-            work_in_lane = kv_work(a, in_lane);
-        }
+    KvPace pace{0, a.whole ? 0 : (end - at) / 4};
+    for (; at < end && window < a.requests; window += 64, k0 = 0) {
+        if (a.direct || !few) look(window + lane);
         const int last_lane = 63 < a.requests - 1 - window ? 63 : a.requests - 1 - window;
-        for (int k = 0; k <= last_lane && at < end; ++k) {
+        for (int k = k0; k <= last_lane && at < end; ++k) {
             const KvWork wk{__builtin_amdgcn_readlane(work_in_lane.units, k), __builtin_amdgcn_readlane(work_in_lane.groups, k)};
             if (wk.groups == 0) continue;
             const int r = window + k;
             const KvSeq s{__builtin_amdgcn_readlane(in_lane.row0, k), __builtin_amdgcn_readlane(in_lane.fresh, k),
                           __builtin_amdgcn_readlane(in_lane.len, k), __builtin_amdgcn_readlane(in_lane.keys, k)};
-            const int per = a.whole ? 1 : wk.units;
+            const int per = a.whole ? 1 : wk.per();
             for (int grp = (at - number) / per; grp < wk.groups && at < end; ++grp) {
                 const int item0 = number + grp * per;
                 const int stop = end < item0 + per ? end : item0 + per;
-                const int u0 = a.whole ? 0 : at - item0, u1 = a.whole ? wk.units : stop - item0;
+                // an item's first numbers are its beginning, those behind them its units
+                const int before = item0 + KV_ITEM_UNITS;
+                const int u0 = a.whole || at < before ? 0 : at - before, u1 = a.whole ? wk.units : stop - before;
+                if (u1 <= u0) {
+                    at = stop;
+                    continue;
+                }
                 const bool complete = u0 == 0 && u1 == wk.units;
                 const int place = u0 == 0 && !complete && at != first_number ? 1 : 0;
                 const int c0 = grp * 16 * CT, columns = s.fresh * a.group;
+                pace.at(a.whole ? u1 : end - at);
                 KvWave<NB, CT, NT, 2> wv;
                 wv.begin(a, s, head, c0, reinterpret_cast<unsigned short*>(&s_acc[wave][0][0]));
-                wv.template walk<kv_decode_depth(NB, CT, NT)>(a, r, head, 4 * u0 + wave, 4 * u1, 4);
+                wv.walk(a, r, head, 4 * u0 + wave, 4 * u1, 4, pace);
                 // join the four waves: one tile of columns and up to four blocks at a time
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
@@ -906,6 +955,8 @@ void kv_decode_kernel(KvAttnArgs a) {
                         }
                     }
                 }
+                if (u0 == 0 && !a.whole && head == 0 && threadIdx.x == 0)
+                    a.spans[kv_item(a, s, r) + grp] = kv_i32x2{2 * share + place, deal.of(item0 + per - 1)};
                 at = stop;
             }
             number += per * wk.groups;
@@ -1007,22 +1058,13 @@ __global__ __launch_bounds__(TPB) void kv_join_kernel(KvAttnArgs a) {
         if (row >= s.fresh) return;
         row += s.row0;
     }
-    int mine = 0, mine_before = 0;
-    for (int k = threadIdx.x; k < a.requests; k += TPB) {
-        const int n = kv_work(a, kv_seq(a, k)).count();
-        mine += n;
-        if (k < r) mine_before += n;
-    }
-    const int total = block_sum(mine, s_wave), before = block_sum(mine_before, s_wave);
-    const int c = (int)(row - s.row0) * a.group + qh % a.group, grp = c / a.tile_columns, col = c % a.tile_columns;
-    const int item0 = before + grp * wk.units, item1 = item0 + wk.units;
-    const KvShares deal(total, a.shares);
-    const int w0 = deal.of(item0), w1 = deal.of(item1 - 1);
+    const int c = (int)(row - s.row0) * a.group + qh % a.group, grp = c >> a.item_shift, col = c & ((1 << a.item_shift) - 1);
+    // as the workgroup that begins the item left it: two for its share and which of the share's places, and the last share
+    const kv_i32x2 span = a.spans[kv_item(a, s, r) + grp];
+    const int w0 = uniform(span[0]) >> 1, place0 = uniform(span[0]) & 1, w1 = uniform(span[1]);
     if (w0 == w1) return;                                // written by the workgroup that had all of it
     const int parts = w1 - w0 + 1;
-    const auto part_row = [&](int k) {
-        return kv_part_row(a, w0 + k, head, item0 > deal.begin(w0 + k) ? 1 : 0, col);
-    };
+    const auto part_row = [&](int k) { return kv_part_row(a, w0 + k, head, k == 0 ? place0 : 0, col); };
     // maxima and sums of all parts at once
     float m = KV_NOTHING;
     for (int k = threadIdx.x; k < parts; k += TPB) {

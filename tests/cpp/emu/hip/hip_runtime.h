@@ -393,6 +393,7 @@ inline float emu_rcpf(float x) {
 #define __builtin_amdgcn_exp2f emu_exp2f
 #define __builtin_amdgcn_rcpf emu_rcpf
 #define __builtin_amdgcn_sched_barrier(mask) ((void)0)
+#define __builtin_amdgcn_s_setprio(priority) ((void)0)
 
 // v_permlane16_swap_b32: the first operand of the lanes 16-31 / 48-63 trades places with the second operand of
 // the lanes 0-15 / 32-47 (lane L + 16 with lane L)
