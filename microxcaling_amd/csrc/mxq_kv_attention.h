@@ -231,7 +231,8 @@ struct KvValues {                                        // .. and values
 
 // Waves that share a SIMD take their turns by priority, then by age: left to age alone, the oldest workgroup of a compute
 // unit is done long before the youngest, which then has nobody to hide its waits behind.  So a wave lowers its priority
-// with every quarter of its work (64 requests with 1900 tokens on average, 8 x 4 heads of 128: 36.7 -> 34.6 us).
+// with every quarter of its work (64 requests with 1900 tokens on average, 8 x 4 heads of 128: 36.7 -> 34.6 us; the
+// prompts below: 84.0 -> 75.5).
 struct KvPace {
     int left, quarter;                                   // units of work, a tile of the wave each
     __device__ __forceinline__ void at(int units_left) {
@@ -612,6 +613,9 @@ constexpr int kv_prompt_ct(int nb, int terms) {
 // tokens, and the join kernel adds its parts.  Numbers are closed forms of the group, so a place is found without a table.
 // One workgroup of the decode kernel's launch, which comes first, works the stretches out (kv_plan), the same for every
 // head: in the prompt kernel itself their arithmetic in 64 bits would hold registers that its loop needs.
+// Tokens that beginning and ending an item counts for (three requests of 1024, 768 and 256 tokens behind 64, 256 and 4096,
+// 8 x 4 heads of 128: 82.6 us with 64, 75.5 with 192, 78.1 with 320).
+constexpr int KV_PROMPT_BEGIN = 192;
 struct KvPrompt {
     int groups;
     int64_t first;                                       // what group 0 counts; a later one `step` more than the one before
@@ -631,7 +635,7 @@ __device__ __forceinline__ KvPrompt kv_prompt(const KvAttnArgs& a, const KvSeq& 
     const int columns = s.fresh * a.group;
     if (columns == 0 || columns <= a.decode_columns) return KvPrompt{0, 0, 0};
     const int64_t seen = a.causal ? (s.len > s.fresh ? s.len - s.fresh : 0) : s.keys;
-    return KvPrompt{(columns + cols - 1) / cols, (seen + 64) * a.group + (a.causal ? cols / 2 : 0), a.causal ? cols : 0};
+    return KvPrompt{(columns + cols - 1) / cols, (seen + KV_PROMPT_BEGIN) * a.group + (a.causal ? cols / 2 : 0), a.causal ? cols : 0};
 }
 struct KvStretch {
     int64_t each, more;
@@ -669,14 +673,14 @@ struct KvPiece {                                         // of an item, for a wo
 struct KvPlanView {
     int* head;                                           // items, shares
     int* items;                                          // of each item: first and last share that it lies in
-    int* shares;                                         // of each share: its first piece, number of pieces
+    int* shares;                                         // of each share: its first piece, number of pieces, tiles of them all
     KvPiece* pieces;                                     // of item i in share w: at i + w
     int64_t* first;                                      // of each request: its first number
     int* item;                                           // .. and its first item
 };
 // (items + shares pieces; 16-byte pieces first)
 __host__ __device__ __forceinline__ int64_t kv_plan_bytes(int64_t items, int64_t shares, int64_t requests) {
-    return 16 * (items + shares) + 8 * requests + 4 * (2 + 2 * items + 2 * shares + requests);
+    return 16 * (items + shares) + 8 * requests + 4 * (2 + 2 * items + 3 * shares + requests);
 }
 __device__ __forceinline__ KvPlanView kv_plan_view(const KvAttnArgs& a) {
     KvPlanView v;
@@ -685,7 +689,7 @@ __device__ __forceinline__ KvPlanView kv_plan_view(const KvAttnArgs& a) {
     v.head = reinterpret_cast<int*>(v.first + a.requests);
     v.items = v.head + 2;
     v.shares = v.items + 2 * (int64_t)a.prompt_items;
-    v.item = v.shares + 2 * (int64_t)a.prompt_shares;
+    v.item = v.shares + 3 * (int64_t)a.prompt_shares;
     return v;
 }
 __device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* s_wave64, int* s_wave) {
@@ -722,7 +726,7 @@ __device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* 
             if (v.first[mid] <= from) lo = mid;
             else hi = mid;
         }
-        int begun = -1, count = 0;
+        int begun = -1, count = 0, all_tiles = 0;
         for (int r = lo; r < a.requests; ++r) {
             const int64_t number = v.first[r];
             if (number >= to) break;
@@ -741,10 +745,12 @@ __device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* 
                 }
                 if (begun < 0) begun = item + w;
                 ++count;
+                all_tiles += tile1 - tile0;
             }
         }
-        v.shares[2 * w] = begun;
-        v.shares[2 * w + 1] = count;
+        v.shares[3 * w] = begun;
+        v.shares[3 * w + 1] = count;
+        v.shares[3 * w + 2] = all_tiles;
     }
 }
 
@@ -1133,7 +1139,10 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g4 = lane >> 4, i16 = lane & 15;
     const KvPlanView plan = kv_plan_view(a);
     if (w >= plan.head[1]) return;
-    const int piece0 = uniform(plan.shares[2 * w]), piece1 = piece0 + uniform(plan.shares[2 * w + 1]);
+    const int piece0 = uniform(plan.shares[3 * w]), piece1 = piece0 + uniform(plan.shares[3 * w + 1]);
+    const int all_tiles = uniform(plan.shares[3 * w + 2]);
+    KvPace pace{0, all_tiles / 4};
+    pace.at(all_tiles);
     for (int at_piece = piece0; at_piece < piece1; ++at_piece) {
         const KvPiece piece = plan.pieces[at_piece];
         const int r = uniform(piece.request), flags = uniform(piece.group_flags), grp = flags >> 2;
@@ -1219,6 +1228,7 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
         __syncthreads();
         for (int tile = tile0; tile < tile1; ++tile) {
             const int buffer = (tile - tile0) & 1;
+            pace.tile();
             if (tile + 1 < tile1) {
                 decode(tile + 1, buffer ^ 1);
                 if (tile + 2 < tile1) load(tile + 2);
