@@ -362,8 +362,8 @@ int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* s
  * out = softmax(scale * q K^T) V, lse = log of the sum of exponentials (may be NULL).  Query head h reads kv head
  * h / (q_heads / heads).  Request r's rows are starts[r] .. starts[r + 1] - 1 (starts NULL: row r), the last of its
  * seq_lens[r] tokens; with causal a row sees the tokens up to its own.  Tokens on pages that do not exist are not
- * seen; a row that sees nothing gets zeros and lse -inf.  Rows behind the last request are left as they are, or
- * zeroed (lse -inf) with zero_tail.  max_new: the most rows of a request, a hint that only steers the choice of
+ * seen; a row that sees nothing gets zeros and lse -inf.  Rows of no request are left as they are, or
+ * zeroed with zero_tail; their lse is -inf.  max_new: the most rows of a request, a hint that only steers the choice of
  * kernels.  workspace: mxq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned. */
 int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
                         int64_t out_head_stride, float* lse, int dtype, int64_t rows, int q_heads, const int* block_table,

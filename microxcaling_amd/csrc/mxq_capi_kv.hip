@@ -193,7 +193,7 @@ int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* s
 
 int64_t mxq_kv_attention_workspace_bytes(int64_t requests, int64_t rows, int q_heads, int64_t max_new, int64_t width, int heads,
                                          int page_size, int head_dim, int dtype) {
-    if (requests <= 0 || rows <= 0 || heads <= 0 || q_heads < heads || width < 0 || page_size <= 0 || head_dim < 1 ||
+    if (requests < 0 || rows <= 0 || heads <= 0 || q_heads < heads || width < 0 || page_size <= 0 || head_dim < 1 ||
         head_dim > 32 * KV_MAX_NB)
         return 0;
     const int terms = dtype == MXQ_DTYPE_F16 ? 2 : 1;

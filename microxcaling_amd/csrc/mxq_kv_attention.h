@@ -714,7 +714,7 @@ __device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* 
     __syncthreads();
     const KvStretch deal(a, total);
     if (threadIdx.x == 0) {
-        v.head[0] = items;
+        v.head[0] = items < 0 || items > a.prompt_items ? a.prompt_items : items;
         v.head[1] = total > 0 ? deal.shares : 0;
     }
     if (total == 0) return;
@@ -735,6 +735,7 @@ __device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* 
             if (p.groups == 0) continue;
             for (int g = from > number ? p.group_of(from - number) : 0; g < p.groups && number + p.begin(g) < to; ++g) {
                 const int tiles = kv_prompt_tiles(a, s, g, cols), item = v.item[r] + g;
+                if ((uint32_t)item >= (uint32_t)a.prompt_items) break;       // (starts that are not in order name rows twice)
                 const int tile0 = kv_prompt_cut(p, g, tiles, from - number), tile1 = kv_prompt_cut(p, g, tiles, to - number);
                 const bool begins = number + p.begin(g) >= from;
                 const bool whole = tile1 - tile0 == tiles && (tiles > 0 || begins);
@@ -800,13 +801,17 @@ void kv_decode_kernel(KvAttnArgs a) {
     const int head = blockIdx.x % a.c.heads, share = blockIdx.x / a.c.heads;
     const int wave = uniform(threadIdx.x >> 6);
 
-    if (a.zero_tail && a.starts) {                       // rows behind the last request of a new output
-        int64_t tail = a.starts[a.requests];
-        tail = tail < 0 ? 0 : tail;
-        const int heads = a.c.heads * a.group;
-        for (int64_t e = tail * heads + blockIdx.x; e < a.rows * heads; e += gridDim.x) {
+    if ((a.zero_tail || a.lse) && a.starts) {            // rows before the first request and behind the last one
+        const int rows = (int)a.rows;
+        int head_rows = a.starts[0], tail = a.starts[a.requests];
+        head_rows = head_rows < 0 ? 0 : (head_rows < rows ? head_rows : rows);
+        tail = tail < head_rows ? head_rows : (tail < rows ? tail : rows);
+        const int heads = a.c.heads * a.group, nobodys = (head_rows + rows - tail) * heads;
+        for (int x = blockIdx.x; x < nobodys; x += gridDim.x) {              // (rows x heads: below 2^31, and so is a step further)
+            const int e = x < head_rows * heads ? x : x + (tail - head_rows) * heads;
             unsigned short* o = kv_out_row(a, e / heads, e % heads);
-            for (int d = threadIdx.x; d < a.c.head_dim; d += TPB) o[d] = 0;
+            if (a.zero_tail)
+                for (int d = threadIdx.x; d < a.c.head_dim; d += TPB) o[d] = 0;
             if (a.lse && threadIdx.x == 0) a.lse[e] = -__builtin_inff();
         }
     }
@@ -1067,8 +1072,10 @@ __global__ __launch_bounds__(TPB) void kv_join_kernel(KvAttnArgs a) {
     const int c = (int)(row - s.row0) * a.group + qh % a.group, grp = c >> a.item_shift, col = c & ((1 << a.item_shift) - 1);
     // as the workgroup that begins the item left it: two for its share and which of the share's places, and the last share
     const kv_i32x2 span = a.spans[kv_item(a, s, r) + grp];
-    const int w0 = uniform(span[0]) >> 1, place0 = uniform(span[0]) & 1, w1 = uniform(span[1]);
-    if (w0 == w1) return;                                // written by the workgroup that had all of it
+    const int place0 = uniform(span[0]) & 1;
+    const uint32_t last_share = (uint32_t)(a.shares - 1);                    // (in bounds also where starts are not in order)
+    const int w0 = (int)min((uint32_t)uniform(span[0]) >> 1, last_share), w1 = (int)min((uint32_t)uniform(span[1]), last_share);
+    if (w1 <= w0) return;                                // written by the workgroup that had all of it
     const int parts = w1 - w0 + 1;
     const auto part_row = [&](int k) { return kv_part_row(a, w0 + k, head, k == 0 ? place0 : 0, col); };
     // maxima and sums of all parts at once

@@ -200,7 +200,7 @@ def _check_append(cache, k, v, slots, round):
 def kv_append(cache, k, v, slots, scale_bits=8, round="nearest", flush_fp32_subnorms=False):
     """Quantizes rows k, v (rows, heads, head_dim; any strides with contiguous elements) as pack_mx does and stores them
     at `slots` (int64, one a row) of the cache, in place.  Rows whose slot is negative or beyond the cache are left out.
-    No slot may be named twice in a call: which row it would then hold is not defined.  fp16 rows need
+    No slot may be named twice in a call: what it would then hold is not defined.  fp16 rows need
     custom_extensions.set_exponent_mode('exact'), as for pack_mx."""
     who = "kv_append"
     data, page_size, head_dim = cache
@@ -259,7 +259,7 @@ def _check_attention(q, cache, block_table, seq_lens, starts, out):
         raise RuntimeError("%s: without starts every request has one row: %d rows, %d requests" % (who, q.shape[0], R))
     if q.shape[0] * q.shape[1] > 0x7FFFFF00:
         raise RuntimeError("%s: q has too many rows" % who)
-    _check_no_grad(who, q)
+    _check_no_grad(who, q, *(() if out is None else (out,)))
     if out is not None:
         _check_rows(out, "out", who)
         _check_on(out, data, "out", who)
@@ -277,8 +277,9 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
     seq_lens (int32): tokens of each request, the new ones (already appended) included.  starts (int32, requests + 1):
     request r has the rows starts[r] .. starts[r + 1] - 1, which are its last tokens; None: one row a request.  With
     causal a row sees the tokens up to its own, otherwise all of its request.  Tokens whose page is not in the cache are
-    not seen.  A row that sees no token gets zeros (lse -inf).  Rows behind the last request are zero (lse -inf) in a new
-    output and left as they are in a given `out`.  scale defaults to head_dim ** -0.5.
+    not seen.  A row that sees no token gets zeros (lse -inf).  Rows of no request (before the first one's and behind the
+    last one's) are zero in a new output and left as they are in a given `out`; their lse is -inf.  scale defaults to
+    head_dim ** -0.5.
 
     max_new: the most rows that a request has, if known: it steers the choice of kernels, never the result.  return_lse:
     also the logarithm of the sum of exponentials, fp32 (rows, query heads).  Accumulation, maxima and sums are fp32; the

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from helpers import assert_bits_equal
+from microxcaling_amd import _lib
 from microxcaling_amd import custom_extensions as ce
 from microxcaling_amd.kv_cache import (PackedKVCache, kv_append, kv_attention, kv_block_tables, kv_read, new_kv_cache)
 from oracle import mx_oracle as O
@@ -443,6 +444,51 @@ def test_rows_behind_the_last_request_and_given_outputs():
     proj[:, :, 73:] = s.q.to(DEV).transpose(0, 1)
     again = s.call(q=proj[:, :, 73:].transpose(0, 1), max_new=3)
     assert torch.equal(again[0], s.call(max_new=3)[0])
+
+
+def test_rows_of_no_request():
+    """Steps without requests, rows before the first request and behind the last one: zero in a new output, as they were
+    in a given one; their lse is -inf in both."""
+    s = Setup([40, 19], [3, 2], 1, 4, 72, 16, seed=19)
+    q = torch.cat([torch.full((2, 4, 72), float("nan"), dtype=s.q.dtype), s.q, s.q[:3]]).to(DEV)
+    starts, want = (s.starts + 2).to(DEV), s.call(max_new=3)
+    for hint in (3, 200):
+        for out in (None, torch.full_like(q, 7.0)):
+            got, lse = kv_attention(q, s.cache, s.table.to(DEV), s.seq.to(DEV), starts, max_new=hint, out=out, return_lse=True)
+            rest = torch.cat([got[:2], got[7:]])
+            assert (rest == (0 if out is None else 7)).all() and (torch.cat([lse[:2], lse[7:]]) == -math.inf).all()
+            if hint == 3:
+                assert torch.equal(got[2:7], want[0]) and torch.equal(lse[2:7], want[1])
+    none, table = torch.zeros(0, dtype=torch.int32, device=DEV), torch.zeros((0, 100), dtype=torch.int32, device=DEV)
+    for hint in (None, 1, 200):
+        got, lse = kv_attention(q, s.cache, table, none, torch.zeros(1, dtype=torch.int32, device=DEV), max_new=hint, return_lse=True)
+        assert not got.any() and (lse == -math.inf).all()
+    got, lse = kv_attention(q[:0], s.cache, table, none, return_lse=True)
+    assert got.shape == (0, 4, 72) and lse.shape == (0, 4)
+    # requests whose tables have no columns see nothing
+    got, lse = s.call(max_new=3)[0] * 0, kv_attention(q[2:7], s.cache, s.table.to(DEV)[:, :0].contiguous(), s.seq.to(DEV), s.starts.to(DEV), return_lse=True)
+    assert torch.equal(lse[0], got) and (lse[1] == -math.inf).all()
+
+
+@pytest.mark.parametrize("starts", [[0, 300, 0, 300, 0, 300], [-5, 300, 7, 2 ** 31 - 1, -2 ** 31, 280], [400, 300, 200, 100, 50, 0]])
+@pytest.mark.parametrize("hint", [1, 300])
+def test_starts_that_are_not_in_order_stay_in_bounds(starts, hint):
+    """Rows named twice get one of the requests' results; nothing outside the tensors and the workspace is written."""
+    s = Setup([300, 20, 90, 260, 5], [1] * 5, 1, 4, 32, 16, seed=20, spare=30)
+    q = torch.randn(300, 4, 32, generator=gen(21)).to(s.q.dtype).to(DEV)
+    lib, st = _lib.gpu(), torch.tensor(starts, dtype=torch.int32).to(DEV)
+    table, seq = s.table.to(DEV), s.seq.to(DEV)
+    need = lib.mxq_kv_attention_workspace_bytes(5, 300, 4, hint, table.shape[1], 1, 16, 32, ce._DTYPE[q.dtype])
+    pad = 1 << 16
+    ws = torch.full((need + 2 * pad,), 0xA5, dtype=torch.uint8, device=DEV)
+    out = torch.zeros((302, 4, 32), dtype=q.dtype, device=DEV)
+    rc = lib.mxq_kv_attention_mx(q.data_ptr(), 128, 32, out[1:].data_ptr(), 128, 32, None, ce._DTYPE[q.dtype], 300, 4, table.data_ptr(),
+                                 table.stride(0), table.shape[1], seq.data_ptr(), st.data_ptr(), 5, 0.2, 1, hint, 0,
+                                 s.cache.data.data_ptr(), s.cache.data.shape[0], 1, 16, 32, ws[pad:].data_ptr(), need, None)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert (ws[:pad] == 0xA5).all() and (ws[pad + need:] == 0xA5).all()
+    assert not out[0].any() and not out[-1].any()
 
 
 def test_refusals():
