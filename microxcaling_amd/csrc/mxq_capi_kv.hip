@@ -31,10 +31,7 @@ int make_cache(void* data, int64_t num_pages, int heads, int page_size, int head
     c->head_dim = head_dim;
     c->nb = (head_dim + 31) / 32;
     c->record = (int64_t)page_size * c->nb * KV_TOKEN_BYTES;
-    int log = 0;                                         // multiply instead of dividing by page_size, exact for 32 bits
-    while ((1 << log) < page_size) ++log;
-    c->divide_by = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << log) - page_size)) / page_size + 1);
-    c->shift_by = (uint32_t)(log - 1);
+    c->by_page = kv_divide((uint32_t)page_size);
     int64_t total;
     if (mul_overflows(num_pages, heads, c->record, &total)) return fail(MXQ_ERR_ARGUMENT, "%s: size overflows int64", who);
     return MXQ_OK;
@@ -247,6 +244,9 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.starts = starts;
     a.requests = (int)requests;
     a.group = q_heads / heads;
+    a.by_group = kv_divide((uint32_t)a.group);
+    a.by_heads = kv_divide((uint32_t)heads);
+    a.by_q_heads = kv_divide((uint32_t)q_heads);
     a.rows = rows;
     a.scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
     if (a.scale_log2 < 1.17549435e-38f) a.scale_log2 = 1.17549435e-38f;      // 0 times a masked score of -inf would be NaN
@@ -260,10 +260,11 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.whole = p.whole ? 1 : 0;
     a.direct = p.whole && !starts && a.group <= 16 * p.ct ? 1 : 0;
     a.shares = (int)p.shares;
+    a.by_shares = kv_divide((uint32_t)a.shares);
     a.join_rows = p.prompt ? p.decode_columns / a.group : 0;
     a.part = reinterpret_cast<float*>(workspace);
     unsigned char* behind = reinterpret_cast<unsigned char*>(workspace) + decode_part_bytes(p, heads);
-    a.spans = reinterpret_cast<kv_i32x2*>(behind);
+    a.spans = reinterpret_cast<int*>(behind);
     behind += span_bytes(p);
     a.prompt_part = p.prompt ? reinterpret_cast<float*>(behind) : nullptr;
     a.plan = p.prompt ? behind + prompt_part_bytes(p, heads, terms) : nullptr;

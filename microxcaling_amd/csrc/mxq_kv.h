@@ -33,17 +33,29 @@ typedef __bf16 kv_bf16x2 __attribute__((ext_vector_type(2)));
 constexpr int KV_MAX_NB = 8;                             // head_dim up to 256
 constexpr int KV_TOKEN_BYTES = 34;                       // bytes of a token's K and V for each block of 32
 
+// Division of 32-bit numbers by one that the host knows: five instructions instead of forty.
+struct KvDivide {
+    uint32_t by, first, then;                            // n / d = (h + (n - h >> first)) >> then, h = high half of n by
+    __device__ __forceinline__ uint32_t of(uint32_t n) const {
+        const uint32_t h = (uint32_t)(((uint64_t)n * by) >> 32);
+        return (h + ((n - h) >> first)) >> then;
+    }
+    __device__ __forceinline__ int of(int n) const { return (int)of((uint32_t)n); }          // n >= 0
+};
+inline KvDivide kv_divide(uint32_t d) {                  // exact: by = 2^32 (2^l - d) / d + 1 with l the first 2^l >= d
+    int l = 0;
+    while (((uint64_t)1 << l) < d) ++l;
+    return KvDivide{(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1), l > 0 ? 1u : 0u, l > 0 ? (uint32_t)(l - 1) : 0u};
+}
+
 struct KvCache {
     unsigned char* data;
     int64_t num_pages;
     int64_t record;                                      // bytes of a (page, head)
     int heads, page_size, head_dim, nb;
-    uint32_t divide_by, shift_by;                        // n / page_size = (h + (n - h >> 1)) >> shift_by, h = high half of n divide_by
+    KvDivide by_page;                                    // by page_size
 };
-__device__ __forceinline__ uint32_t kv_page_of(const KvCache& c, uint32_t n) {
-    const uint32_t h = (uint32_t)(((uint64_t)n * c.divide_by) >> 32);
-    return (h + ((n - h) >> 1)) >> c.shift_by;
-}
+__device__ __forceinline__ uint32_t kv_page_of(const KvCache& c, uint32_t n) { return c.by_page.of(n); }
 
 // ---- exchanges between the four lane groups of 16 -------------------------------------------------------------
 // f(v of this lane, v of lane ^ 16), then the same with lane ^ 32: a reduction over the groups, in every lane

@@ -32,6 +32,7 @@ struct KvAttnArgs {
     const int* seq_lens;
     const int* starts;                                   // (requests + 1), or null: one row a request
     int requests, group;                                 // query heads of a kv head
+    KvDivide by_group, by_heads, by_q_heads, by_shares;
     int64_t rows;                                        // rows of q and out
     float scale_log2;                                    // |scale| log2(e)
     int negative;                                        // scale is
@@ -42,7 +43,7 @@ struct KvAttnArgs {
     int direct;                                          // .. and one item for each request
     int shares;                                          // decode: workgroups of a kv head, at most KV_MAX_SHARES
     int join_rows;                                       // join: so many rows of each request, or 0: every row
-    kv_i32x2* spans;                                     // decode: where the parts of each item lie (KvSpan)
+    int* spans;                                          // decode: where the parts of each item lie (two numbers, KvShares)
     float* part;                                         // decode: partial results, two places for each workgroup
     int join_blocks;                                     // join: workgroups for decode rows, the others for prompt items
     int prompt_shares, prompt_items;                     // prompt: workgroups of a kv head and items of it, at most
@@ -269,8 +270,8 @@ struct KvWave {
         g = lane >> 4;
         const int columns = s.fresh * a.group;
         const int last = (c0 + 16 * CT < columns ? c0 + 16 * CT : columns) - 1;
-        min_limit = kv_limit(a, s, c0 / a.group);
-        max_limit = kv_limit(a, s, last / a.group);
+        min_limit = kv_limit(a, s, a.by_group.of(c0));
+        max_limit = kv_limit(a, s, a.by_group.of(last));
         started = false;
         limits = 0;
 #pragma unroll
@@ -279,7 +280,7 @@ struct KvWave {
             l[ct] = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[ct][b][0] = acc[ct][b][1] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            const int c = c0 + 16 * ct + i16, token = c / a.group;
+            const int c = c0 + 16 * ct + i16, token = a.by_group.of(c);
             const bool live = c < columns;
             limits |= (uint32_t)((live ? kv_limit(a, s, token) : max_limit) - min_limit) << (8 * ct);   // (at most 16 CT tokens apart)
             const unsigned short* row = a.q + (int64_t)(s.row0 + (live ? token : 0)) * a.q_token +
@@ -288,7 +289,7 @@ struct KvWave {
                 __syncthreads();                         // what was there has been read
 #pragma nounroll
                 for (int e = here_only(lane); e < 16 * 32 * NB; e += 64) {
-                    const int x = c0 + 16 * ct + e / (32 * NB), d = e % (32 * NB), t = x / a.group;
+                    const int x = c0 + 16 * ct + e / (32 * NB), d = e % (32 * NB), t = a.by_group.of(x);
                     unsigned short v = 0;
                     if (x < columns && d < a.c.head_dim)
                         v = a.q[(int64_t)(s.row0 + t) * a.q_token + ((int64_t)head * a.group + (x - t * a.group)) * a.q_head + d];
@@ -461,7 +462,7 @@ struct KvWave {
         bool there;
     };
     __device__ __forceinline__ static Spot spot(const KvAttnArgs& a, const int* row, int head, int sub, int end) {
-        const int subs = a.c.page_size / 16, at = sub / subs;
+        const int subs = a.c.page_size / 16, at = (int)kv_page_of(a.c, 16u * (uint32_t)sub);
         int page = -1, in_page = 0;
         if (at < a.width && sub < end) {
             page = row[at];
@@ -657,7 +658,7 @@ struct KvStretch {
 __device__ __forceinline__ int kv_prompt_tiles(const KvAttnArgs& a, const KvSeq& s, int g, int cols) {
     const int columns = s.fresh * a.group;
     const int last = ((g + 1) * cols < columns ? (g + 1) * cols : columns) - 1;
-    return (kv_limit(a, s, last / a.group) + 63) / 64;
+    return (kv_limit(a, s, a.by_group.of(last)) + 63) / 64;
 }
 __device__ __forceinline__ int kv_prompt_cut(const KvPrompt& p, int g, int tiles, int64_t x) {
     const int64_t b = p.begin(g), e = p.begin(g + 1);
@@ -764,12 +765,8 @@ __device__ __forceinline__ void kv_plan(const KvAttnArgs& a, int cols, int64_t* 
 struct KvShares {
     int each = 0, more = 0;
     KvShares() = default;
-    __device__ __forceinline__ KvShares(int units, int shares) : each(units / shares), more(units - units / shares * shares) {}
+    __device__ __forceinline__ KvShares(const KvAttnArgs& a, int units) : each(a.by_shares.of(units)), more(units - each * a.shares) {}
     __device__ __forceinline__ int begin(int w) const { return w * each + (w < more ? w : more); }
-    __device__ __forceinline__ int of(int unit) const {
-        const int big = more * (each + 1);
-        return unit < big ? unit / (each + 1) : more + (unit - big) / each;
-    }
 };
 
 // The first item (16 CT columns of a request) of request r, in an order that needs no sums over requests: every item has a
@@ -798,7 +795,7 @@ void kv_decode_kernel(KvAttnArgs a) {
         kv_plan(a, 64 * kv_prompt_ct(NB, NT), s_wave64, s_wave);
         return;
     }
-    const int head = blockIdx.x % a.c.heads, share = blockIdx.x / a.c.heads;
+    const int share = a.by_heads.of((int)blockIdx.x), head = (int)blockIdx.x - share * a.c.heads;
     const int wave = uniform(threadIdx.x >> 6);
 
     if ((a.zero_tail || a.lse) && a.starts) {            // rows before the first request and behind the last one
@@ -842,7 +839,7 @@ void kv_decode_kernel(KvAttnArgs a) {
         }
         const int total = __builtin_amdgcn_readlane(upto, 63);
         if (!a.whole) {
-            deal = KvShares(total, a.shares);
+            deal = KvShares(a, total);
             at = deal.begin(share);
             end = deal.begin(share + 1);
         }
@@ -858,7 +855,7 @@ void kv_decode_kernel(KvAttnArgs a) {
             total += block_sum(rest, s_wave);
         }
         if (!a.whole) {
-            deal = KvShares(total, a.shares);
+            deal = KvShares(a, total);
             at = deal.begin(share);
             end = deal.begin(share + 1);
         }
@@ -891,12 +888,13 @@ void kv_decode_kernel(KvAttnArgs a) {
             const KvSeq s{__builtin_amdgcn_readlane(in_lane.row0, k), __builtin_amdgcn_readlane(in_lane.fresh, k),
                           __builtin_amdgcn_readlane(in_lane.len, k), __builtin_amdgcn_readlane(in_lane.keys, k)};
             const int per = a.whole ? 1 : wk.per();
-            for (int grp = (at - number) / per; grp < wk.groups && at < end; ++grp) {
+            for (int grp = wk.groups > 1 ? max((at - number) / per, 0) : 0; grp < wk.groups && at < end; ++grp) {
                 const int item0 = number + grp * per;
                 const int stop = end < item0 + per ? end : item0 + per;
                 // an item's first numbers are its beginning, those behind them its units
                 const int before = item0 + KV_ITEM_UNITS;
-                const int u0 = a.whole || at < before ? 0 : at - before, u1 = a.whole ? wk.units : stop - before;
+                // (between 0 and the item's units also where starts that are not in order let the numbers overflow)
+                const int u0 = a.whole ? 0 : max(at - before, 0), u1 = a.whole ? wk.units : min(stop - before, wk.units);
                 if (u1 <= u0) {
                     at = stop;
                     continue;
@@ -951,8 +949,9 @@ void kv_decode_kernel(KvAttnArgs a) {
                                 const float inv = sum_l == 0.0f ? 0.0f : 1.0f / sum_l;
 #pragma unroll
                                 for (int x = 0; x < 8; ++x) y[x] *= inv;
-                                const int64_t row = s.row0 + c / a.group;
-                                const int64_t qh = (int64_t)head * a.group + c % a.group;
+                                const int token = a.by_group.of(c);
+                                const int64_t row = s.row0 + token;
+                                const int64_t qh = (int64_t)head * a.group + (c - token * a.group);
                                 kv_store8<DT>(a, kv_out_row(a, row, qh), 32 * b0 + d0, y);
                                 if (a.lse && b0 == 0 && d0 == 0) a.lse[row * a.c.heads * a.group + qh] = kv_lse(top, sum_l);
                             } else {
@@ -966,8 +965,11 @@ void kv_decode_kernel(KvAttnArgs a) {
                         }
                     }
                 }
-                if (u0 == 0 && !a.whole && head == 0 && threadIdx.x == 0)
-                    a.spans[kv_item(a, s, r) + grp] = kv_i32x2{2 * share + place, deal.of(item0 + per - 1)};
+                if (!a.whole && head == 0 && threadIdx.x == 0) {             // for the join kernel
+                    int* span = a.spans + 2 * (kv_item(a, s, r) + grp);
+                    if (u0 == 0) span[0] = 2 * share + place;
+                    if (u1 == wk.units) span[1] = share;
+                }
                 at = stop;
             }
             number += per * wk.groups;
@@ -986,7 +988,7 @@ __device__ __forceinline__ float* kv_prompt_part_ml(const KvAttnArgs& a, int64_t
 template <int DT, int NB, int CT>
 __device__ __forceinline__ void kv_prompt_join(const KvAttnArgs& a, int block) {
     constexpr int COLS = 64 * CT, DP = 32 * NB;
-    const int head = block % a.c.heads, sixteen = block / a.c.heads % (4 * CT), item = block / a.c.heads / (4 * CT);
+    const int of_head = a.by_heads.of(block), head = block - of_head * a.c.heads, sixteen = of_head % (4 * CT), item = of_head / (4 * CT);
     const KvPlanView plan = kv_plan_view(a);
     if (plan.head[1] == 0 || item >= plan.head[0]) return;
     const int w0 = plan.items[2 * item], w1 = plan.items[2 * item + 1];
@@ -1024,7 +1026,8 @@ __device__ __forceinline__ void kv_prompt_join(const KvAttnArgs& a, int block) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int x = 0; x < 8; ++x) y[x] *= inv;
-        const int64_t q_row = s.row0 + c / a.group, qh = (int64_t)head * a.group + c % a.group;
+        const int token = a.by_group.of(c);
+        const int64_t q_row = s.row0 + token, qh = (int64_t)head * a.group + (c - token * a.group);
         kv_store8<DT>(a, kv_out_row(a, q_row, qh), d0, y);
         if (a.lse && d0 == 0) a.lse[q_row * a.c.heads * a.group + qh] = kv_lse(m, l);
     }
@@ -1045,8 +1048,8 @@ __global__ __launch_bounds__(TPB) void kv_join_kernel(KvAttnArgs a) {
         return;
     }
     const int q_heads = a.c.heads * a.group;
-    const int qh = blockIdx.x % q_heads, head = qh / a.group;
-    int64_t row = blockIdx.x / q_heads;
+    int64_t row = a.by_q_heads.of(blockIdx.x);
+    const int qh = (int)blockIdx.x - (int)row * q_heads, head = a.by_group.of(qh);
     int r = (int)row;
     if (a.join_rows) {                                   // the first rows of each request: others are the prompt kernel's
         r = (int)(row / a.join_rows);
@@ -1069,9 +1072,9 @@ __global__ __launch_bounds__(TPB) void kv_join_kernel(KvAttnArgs a) {
         if (row >= s.fresh) return;
         row += s.row0;
     }
-    const int c = (int)(row - s.row0) * a.group + qh % a.group, grp = c >> a.item_shift, col = c & ((1 << a.item_shift) - 1);
-    // as the workgroup that begins the item left it: two for its share and which of the share's places, and the last share
-    const kv_i32x2 span = a.spans[kv_item(a, s, r) + grp];
+    const int c = (int)(row - s.row0) * a.group + (qh - head * a.group), grp = c >> a.item_shift, col = c & ((1 << a.item_shift) - 1);
+    // as the workgroups left it that begin and end the item: twice the first share, plus which of its places; the last share
+    const kv_i32x2 span = *reinterpret_cast<const kv_i32x2*>(a.spans + 2 * (kv_item(a, s, r) + grp));
     const int place0 = uniform(span[0]) & 1;
     const uint32_t last_share = (uint32_t)(a.shares - 1);                    // (in bounds also where starts are not in order)
     const int w0 = (int)min((uint32_t)uniform(span[0]) >> 1, last_share), w1 = (int)min((uint32_t)uniform(span[1]), last_share);
@@ -1142,7 +1145,7 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
     using Wave = KvWave<NB, CT, NT, NP>;
     __shared__ uint32_t s_nan[2][2][NB];                 // masked tiles: tokens with a NaN block, by half of 32 tokens
     __shared__ u32x4 s_k[2][4 * NB][64], s_v[2][4 * NB][64];                 // [buffer][operand][lane]
-    const int head = blockIdx.x % a.c.heads, w = blockIdx.x / a.c.heads;
+    const int w = a.by_heads.of((int)blockIdx.x), head = (int)blockIdx.x - w * a.c.heads;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g4 = lane >> 4, i16 = lane & 15;
     const KvPlanView plan = kv_plan_view(a);
     if (w >= plan.head[1]) return;
@@ -1161,7 +1164,7 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
         const int columns = s.fresh * a.group;
         const int wg_c0 = grp * COLS, c0 = wg_c0 + wave * (16 * CT);
         const int wg_last = (wg_c0 + COLS < columns ? wg_c0 + COLS : columns) - 1;
-        const int wg_min = kv_limit(a, s, wg_c0 / a.group), wg_max = kv_limit(a, s, wg_last / a.group);
+        const int wg_min = kv_limit(a, s, a.by_group.of(wg_c0)), wg_max = kv_limit(a, s, a.by_group.of(wg_last));
         const bool works = c0 < columns;         // uniform over the wave
         Wave wv;
         wv.begin(a, s, head, works ? c0 : wg_c0, reinterpret_cast<unsigned short*>(&s_k[0][0][0]) + wave * (16 * 32 * NB));
@@ -1282,7 +1285,8 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
             if (c >= columns) continue;
             if (complete) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int64_t q_row = s.row0 + c / a.group, qh = (int64_t)head * a.group + c % a.group;
+                const int token = a.by_group.of(c);
+        const int64_t q_row = s.row0 + token, qh = (int64_t)head * a.group + (c - token * a.group);
                 unsigned short* o = kv_out_row(a, q_row, qh);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
