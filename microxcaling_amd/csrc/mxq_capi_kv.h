@@ -8,7 +8,7 @@ namespace mxq_kv {
 // what a call of the attention runs
 struct Plan {
     int nb, ct;                    // blocks of a row; column tiles of a decode item
-    bool decode, prompt, whole;
+    bool prompt, whole;
     int decode_columns;
     int64_t decode_items;          // whole: workgroups of a kv head
     int64_t shares;

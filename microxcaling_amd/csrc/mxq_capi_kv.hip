@@ -60,13 +60,22 @@ Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64
     if (max_new > rows) max_new = rows;
     if (max_new < 1) max_new = 1;
     const int64_t columns = max_new * group;
-    p.prompt = columns > 64;
-    p.decode = true;
-    p.decode_columns = p.prompt ? 64 : 0x7FFFFFFF;
-    p.ct = columns <= 16 ? 1 : kv_decode_most_ct(nb, terms);
+    const int most_ct = kv_decode_most_ct(nb, terms);
+    // 30 columns of 96 with two tiles of them for each reading of the tokens 35.9 us, with one 42.6 (16 requests of 4096)
+    p.ct = columns <= 16 ? 1 : most_ct;
+    // The prompt kernel multiplies at up to four times the decode kernel's rate, but takes a plan and a join of many
+    // columns, 20 us of launches.  8 x 4 heads of 128, us with decode and prompt kernel: 4 requests of 2048 with 128, 192,
+    // 256, 384 columns each 32 : 42, 40 : 45, 47 : 48, 62 : 54; 16 of them with 128 and 192 51 : 62, 92 : 67; one of 4096
+    // with 512 39 : 53; one of 16384 with 256 48 : 69; new prompts alone, 512 tokens 18 : 39, 1024 60 : 59.
+    const double work = (double)rows * group * heads * (room + 3 * KV_UNIT) * (2.0 / most_ct);
+    p.prompt = columns > 64 * most_ct && work > 28e6;
+    p.decode_columns = p.prompt ? 64 * most_ct : 0x7FFFFFFF;
     const int64_t units = ceil_div(room, KV_UNIT) > 0 ? ceil_div(room, KV_UNIT) : 1;
     p.decode_items = rows * group / (16 * p.ct) + (requests > 0 ? requests : 1);
-    p.whole = units <= 4;
+    // A workgroup for each item, and no join: 32 requests of 500, 760, 1000, 1500 tokens (8 x 4 heads of 128) 11.3, 13.7, 16.3,
+    // 20.7 us, against 16.6, 17.0, 19.3, 21.8 with the units dealt out; 8 requests 12.2, 13.9, 17.7 against 13.0, 13.9, 14.9
+    // from 760 on; one request 10.5, 12.1, 13.7 against 11.5, 11.7, 11.7.
+    p.whole = units <= 4 || (units <= 8 && requests * heads >= 64);
     const int64_t chip = 256 * kv_decode_waves(nb, p.ct, terms);
     p.shares = ceil_div(chip, heads) < KV_MAX_SHARES ? ceil_div(chip, heads) : KV_MAX_SHARES;
     if (p.shares > p.decode_items * units) p.shares = p.decode_items * units;

@@ -446,6 +446,91 @@ def test_rows_behind_the_last_request_and_given_outputs():
     assert torch.equal(again[0], s.call(max_new=3)[0])
 
 
+def wide_table(new, q_heads, page):
+    """Table entries behind the tokens, as of a server with a long context: what a call could read decides whether
+    requests with many columns take the prompt kernel, and short ones alone would not."""
+    return min(-(-60_000_000 // (sum(new) * q_heads * page)), (1 << 29) // page)
+
+
+def takes_prompt_kernel(s, hint):
+    size = lambda n: _lib.gpu().mxq_kv_attention_workspace_bytes(len(s.lens), s.q.shape[0], s.q.shape[1], n, s.table.shape[1], s.heads,
+                                                                 s.page, s.dim, ce._DTYPE[s.q.dtype])
+    return size(hint) > size(16 // s.group + 1)                   # parts of prompts and a plan
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,new,heads,group,dim,page,causal", [
+    ([100, 35, 0, 64], [70, 1, 0, 64], 2, 2, 64, 16, True), ([150], [101], 1, 4, 128, 48, True), ([140], [130], 1, 1, 80, 16, False),
+    ([90, 77], [70, 77], 1, 1, 256, 16, True), ([90, 8], [60, 8], 1, 3, 96, 32, False), ([180, 140], [150, 140], 1, 1, 33, 16, True),
+    ([81], [66], 1, 2, 200, 16, True), ([70, 300], [70, 1], 1, 3, 160, 16, True)])
+def test_prompt_chunks_in_wide_tables(lens, new, heads, group, dim, page, causal, dtype):
+    s = Setup(lens, new, heads, group, dim, page, dtype, seed=4, spare=wide_table(new, heads * group, page))
+    assert takes_prompt_kernel(s, max(new))
+    first = s.call(max_new=max(new), causal=causal)
+    s.check(first, terms=1 if dtype == torch.bfloat16 else 2, causal=causal)
+    again = s.call(max_new=max(new), causal=causal)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_scales_of_prompt_chunks_in_wide_tables(scale):
+    s = Setup([90, 33], [80, 20], 1, 4, 64, 16, spare=wide_table([100], 4, 16))
+    assert takes_prompt_kernel(s, 80)
+    s.check(s.call(max_new=80, scale=scale), scale=scale, terms=1)
+
+
+def test_prompt_chunks_on_missing_pages_in_wide_tables():
+    s = Setup([130, 96, 90], [70] * 3, 1, 2, 64, 16, seed=12, spare=wide_table([210], 2, 16))
+    assert takes_prompt_kernel(s, 70)
+    s.table[0, 2], s.table[0, 4], s.table[1] = -1, 2 ** 31 - 1, s.cache.data.shape[0]
+    s.table[2, 3:] = -5
+    missing = torch.zeros(130, dtype=torch.bool)
+    missing[32:48] = missing[64:80] = True
+    seen = {0: ~missing, 1: torch.zeros(96, dtype=torch.bool), 2: torch.arange(90) < 48}
+    s.check(s.call(max_new=70), seen=lambda r: seen[r], terms=1)
+
+
+@pytest.mark.parametrize("dim,at", [(64, 41), (128, 130)])
+def test_a_token_with_nan_in_prompt_chunks_in_wide_tables(dim, at):
+    for what in ("v", "k"):
+        runs = []
+        for bad in (False, True):
+            s = Setup([180], [170], 1, 1, dim, 16, seed=14, spare=wide_table([170], 1, 16))
+            assert takes_prompt_kernel(s, 170)
+            if bad:
+                (s.v if what == "v" else s.k)[0][at, 0, 5] = float("inf")
+                kv_append(s.cache, s.k[0].to(DEV), s.v[0].to(DEV), s.slots[0].to(DEV))
+            runs.append([t.cpu() for t in s.call(max_new=170)])
+        (cout, clse), (out, lse) = runs
+        before = at - 10                                          # rows 0 .. see 11 .. tokens
+        assert torch.equal(out[:before], cout[:before]) and torch.equal(lse[:before], clse[:before])
+        if what == "v":
+            assert torch.isnan(out[before:, 0, :32]).all() and torch.equal(out[before:, 0, 32:], cout[before:, 0, 32:])
+            assert torch.equal(lse, clse)
+        else:
+            assert torch.isnan(out[before:]).all() and torch.isnan(lse[before:]).all()
+
+
+def test_rows_and_outputs_of_prompt_chunks_in_wide_tables():
+    """Rows of no request, outputs that are not aligned, queries as a slice with heads before rows."""
+    s = Setup([90, 60, 45], [80, 2, 40], 1, 4, 72, 16, seed=18, spare=wide_table([122], 4, 16))
+    assert takes_prompt_kernel(s, 80)
+    q = torch.cat([s.q, torch.full((4, 4, 72), float("nan"), dtype=s.q.dtype)]).to(DEV)
+    got = s.call(q=q, max_new=80)
+    s.check((got[0][:122], got[1][:122]), terms=1)
+    assert not got[0][122:].any() and (got[1][122:] == -math.inf).all()
+    out = torch.full((126, 4, 80), 7.0, dtype=s.q.dtype, device=DEV)
+    res = s.call(q=q, max_new=80, out=out[:, :, 3:75])
+    assert torch.equal(res[0][:122], got[0][:122]) and torch.equal(res[1], got[1])
+    assert (out[122:] == 7).all() and (out[:, :, :3] == 7).all() and (out[:, :, 75:] == 7).all()
+    proj = torch.zeros(4, 122, 145, dtype=s.q.dtype, device=DEV)
+    proj[:, :, 73:] = s.q.to(DEV).transpose(0, 1)
+    assert torch.equal(s.call(q=proj[:, :, 73:].transpose(0, 1), max_new=80)[0], got[0][:122])
+    none, table = torch.zeros(0, dtype=torch.int32, device=DEV), torch.zeros((0, s.table.shape[1]), dtype=torch.int32, device=DEV)
+    got, lse = kv_attention(q, s.cache, table, none, torch.zeros(1, dtype=torch.int32, device=DEV), max_new=80, return_lse=True)
+    assert not got.any() and (lse == -math.inf).all()
+
+
 def test_rows_of_no_request():
     """Steps without requests, rows before the first request and behind the last one: zero in a new output, as they were
     in a given one; their lse is -inf in both."""
@@ -471,10 +556,10 @@ def test_rows_of_no_request():
 
 
 @pytest.mark.parametrize("starts", [[0, 300, 0, 300, 0, 300], [-5, 300, 7, 2 ** 31 - 1, -2 ** 31, 280], [400, 300, 200, 100, 50, 0]])
-@pytest.mark.parametrize("hint", [1, 300])
-def test_starts_that_are_not_in_order_stay_in_bounds(starts, hint):
+@pytest.mark.parametrize("hint,spare", [(1, 30), (300, 30), (300, 60000)])
+def test_starts_that_are_not_in_order_stay_in_bounds(starts, hint, spare):
     """Rows named twice get one of the requests' results; nothing outside the tensors and the workspace is written."""
-    s = Setup([300, 20, 90, 260, 5], [1] * 5, 1, 4, 32, 16, seed=20, spare=30)
+    s = Setup([300, 20, 90, 260, 5], [1] * 5, 1, 4, 32, 16, seed=20, spare=spare)
     q = torch.randn(300, 4, 32, generator=gen(21)).to(s.q.dtype).to(DEV)
     lib, st = _lib.gpu(), torch.tensor(starts, dtype=torch.int32).to(DEV)
     table, seq = s.table.to(DEV), s.seq.to(DEV)
