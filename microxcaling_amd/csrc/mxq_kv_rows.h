@@ -12,8 +12,8 @@ namespace {
 // pages, in the order of the requests: an exclusive prefix sum.  A thread owns a new token: it finds its request
 // by bisection in the prefix sums of the workgroup's share, its page either in the old part of the table or in the
 // free list (so no thread waits for another one's table entry), and the first token of a page writes the entry.
-// One launch, bound by latency for a decoding step; every workgroup repeats the sums over all requests, which are
-// a few kilobytes.
+// One launch, bound by latency: 4.0 us for a decoding step of one workgroup, 7.1 us for 50000 new tokens; every workgroup
+// repeats the sums over all requests, which are a few kilobytes.
 struct KvTablesArgs {
     const int* context;
     const int* fresh;
@@ -132,7 +132,9 @@ __global__ __launch_bounds__(TPB) void kv_block_tables_kernel(KvTablesArgs a) {
 // block; a group of 16 lanes keeps its head, K or V, and block, and goes through the groups of four tokens.  K's dword
 // goes out as it is.  Of V the four lanes of a quad hold the bytes (i = 4 j .. 4 j + 3) of four tokens; where these
 // tokens are the four of one V tile (every tile of a prompt), they trade bytes and store a dword each, otherwise
-// (decoding steps) four bytes.  Bound by memory for prompts, by latency for single tokens.
+// (decoding steps) four bytes.  Bound by memory for prompts (16384 rows of 8 heads of 128 in bf16 at random slots: 36 us, 66 MB
+// read and 41 MB written for 18, since the bytes of a V tile come at different times; reading them back as fp32 40 us,
+// 4.5 TB/s), by latency for single tokens (3.8 and 3.6 us for a step of 128 rows).
 //
 // Rounding half away from zero with v_cvt_scalef32_pk_fp4_f32, which rounds half to even: values are moved a little
 // further from zero first, so that what lies on a border between two codes lies above it, and nothing else crosses one.
