@@ -235,7 +235,7 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     // units and items are numbered in 32 bits
     const int64_t most_units = (requests + ceil_div(rows * q_heads / heads, 16)) * (ceil_div(width * page_size, KV_UNIT) + 1 + KV_ITEM_UNITS);
     // .. and so are the workgroups of a launch
-    if (most_units > 0x7FFFFFFF || p.prompt_items * heads * 16 + (int64_t)64 * requests * heads > 0x7FFFFFFF || p.decode_items * heads > 0x7FFFFFFF) return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
+    if (most_units > 0x7FFFFFFF || p.prompt_items * heads * 16 + (int64_t)128 * requests * heads > 0x7FFFFFFF || p.decode_items * heads > 0x7FFFFFFF) return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
     if (workspace_bytes < needed || (needed > 0 && !workspace))
         return fail(MXQ_ERR_ARGUMENT, "%s: the workspace is too small", who);
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(MXQ_ERR_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);

@@ -810,8 +810,8 @@ void kv_decode_kernel(KvAttnArgs a) {
         head_rows = head_rows < 0 ? 0 : (head_rows < rows ? head_rows : rows);
         tail = tail < head_rows ? head_rows : (tail < rows ? tail : rows);
         const int heads = a.c.heads * a.group, nobodys = (head_rows + rows - tail) * heads;
-        for (int x = blockIdx.x; x < nobodys; x += gridDim.x) {              // (rows x heads: below 2^31, and so is a step further)
-            const int e = x < head_rows * heads ? x : x + (tail - head_rows) * heads;
+        for (uint32_t x = blockIdx.x; x < (uint32_t)nobodys; x += gridDim.x) {   // (rows x heads and the grid: below 2^31 each)
+            const int e = (int)x < head_rows * heads ? (int)x : (int)x + (tail - head_rows) * heads;
             unsigned short* o = kv_out_row(a, e / heads, e % heads);
             if (a.zero_tail)
                 for (int d = threadIdx.x; d < a.c.head_dim; d += TPB) o[d] = 0;

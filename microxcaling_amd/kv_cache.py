@@ -283,7 +283,7 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
 
     max_new: the most rows that a request has, if known: it steers the choice of kernels, never the result.  return_lse:
     also the logarithm of the sum of exponentials, fp32 (rows, query heads).  Accumulation, maxima and sums are fp32; the
-    probabilities enter the second product as bf16 (two bf16 terms for few rows a request and for fp16 queries)."""
+    probabilities enter the second product as two bf16 terms, or as one for large chunks of bf16 queries."""
     data, page_size, head_dim = cache
     at, shape, table, q_shape, R = data.get_device(), data.shape, block_table.shape, q.shape, seq_lens.numel()
     qs, heads = q.stride(), shape[1] if len(shape) == 3 else 0
