@@ -372,6 +372,17 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
                         int heads, int page_size, int head_dim, void* workspace, int64_t workspace_bytes, void* hip_stream);
 int64_t mxq_kv_attention_workspace_bytes(int64_t requests, int64_t rows, int q_heads, int64_t max_new, int64_t width, int heads,
                                          int page_size, int head_dim, int dtype);
+/* The four calls above with their arguments as 64-bit values in an array, for callers that convert every argument at
+ * a cost (a call through ctypes with 19 of them: 1.9 us, this way 0.7).  args: the arguments in their order without the
+ * stream, addresses and numbers as int64, scale as the bits of a double; of mxq_kv_attention_mx without workspace
+ * and workspace_bytes, which are passed here (the other calls take NULL, 0). */
+#define MXQ_KV_BLOCK_TABLES 0
+#define MXQ_KV_APPEND 1
+#define MXQ_KV_READ 2
+#define MXQ_KV_ATTENTION 3
+int mxq_kv_call(int which, const int64_t* args, void* workspace, int64_t workspace_bytes, void* hip_stream);
+/* mxq_kv_attention_workspace_bytes of the same array as MXQ_KV_ATTENTION takes */
+int64_t mxq_kv_attention_args_workspace_bytes(const int64_t* args);
 
 
 /* ---- libmxq_host.so: the same arithmetic compiled for the host ----------------------------------

@@ -71,6 +71,8 @@ GPU_SYMBOLS = {
                                      _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_f32, _c_int, _c_i64, _c_int,
                                      _c_ptr, _c_i64, _c_int, _c_int, _c_int, _c_ptr, _c_i64, _c_ptr]),
     "mxq_kv_attention_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int]),
+    "mxq_kv_call": (_c_int, [_c_int, ctypes.c_char_p, _c_ptr, _c_i64, _c_ptr]),
+    "mxq_kv_attention_args_workspace_bytes": (_c_i64, [ctypes.c_char_p]),
     "mxq_reduce_sum_inner": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr]),
     "mxq_reduce_max_inner": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr]),
     "mxq_reduce_outer_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),

@@ -1,4 +1,6 @@
 // C ABI of libmxq_gfx950.so, continued: the paged MXFP4 key / value cache.
+#include <cstring>
+
 #include "mxq_capi_kv.h"
 #include "mxq_kv_rows.h"
 
@@ -291,6 +293,36 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     }
     mxq_kv::launch_join(dtype, &a, p, s);
     return check_launch(who);
+}
+
+int mxq_kv_call(int which, const int64_t* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (!a) return fail(MXQ_ERR_ARGUMENT, "mxq_kv_call: null pointer");
+    const auto ints = [&](int n) { return reinterpret_cast<int*>(a[n]); };
+    const auto at = [&](int n) { return reinterpret_cast<void*>(a[n]); };
+    const auto number = [&](int n) { return (int)a[n]; };
+    switch (which) {
+        case MXQ_KV_BLOCK_TABLES:
+            return mxq_kv_block_tables(ints(0), ints(1), ints(2), a[3], a[4], ints(5), a[6], ints(7), a[8], number(9), a[10],
+                                       reinterpret_cast<int64_t*>(a[11]), ints(12), ints(13), ints(14), ints(15), ints(16), hip_stream);
+        case MXQ_KV_APPEND:
+            return mxq_kv_append_mx(at(0), at(1), number(2), a[3], a[4], a[5], a[6], a[7], reinterpret_cast<const int64_t*>(a[8]), at(9),
+                                    a[10], number(11), number(12), number(13), number(14), number(15), number(16), number(17), hip_stream);
+        case MXQ_KV_READ:
+            return mxq_kv_read_mx(at(0), at(1), number(2), a[3], reinterpret_cast<const int64_t*>(a[4]), at(5), a[6], number(7), number(8),
+                                  number(9), hip_stream);
+        case MXQ_KV_ATTENTION: {
+            double scale;
+            memcpy(&scale, &a[16], sizeof scale);
+            return mxq_kv_attention_mx(at(0), a[1], a[2], at(3), a[4], a[5], reinterpret_cast<float*>(a[6]), number(7), a[8], number(9),
+                                       ints(10), a[11], a[12], ints(13), ints(14), a[15], (float)scale, number(17), a[18], number(19),
+                                       at(20), a[21], number(22), number(23), number(24), workspace, workspace_bytes, hip_stream);
+        }
+    }
+    return fail(MXQ_ERR_ARGUMENT, "mxq_kv_call: unknown call %d", which);
+}
+
+int64_t mxq_kv_attention_args_workspace_bytes(const int64_t* a) {
+    return mxq_kv_attention_workspace_bytes(a[15], a[8], (int)a[9], a[18], a[12], (int)a[22], (int)a[23], (int)a[24], (int)a[7]);
 }
 
 }  // extern "C"

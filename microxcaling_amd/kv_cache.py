@@ -10,6 +10,7 @@ Keys and values are quantized along head_dim in blocks of 32 with the arithmetic
 element): what kv_read returns is bit for bit what quantize_mx returns for the same rows.  Lengths, tables, slots and
 starts stay on the GPU, no call waits for it, and every call can be captured into a graph.  Indexes in those tensors
 are checked by the kernels: a slot or a page outside the cache is neither written nor read."""
+import struct
 from typing import NamedTuple
 
 import torch
@@ -86,15 +87,21 @@ def _check_on(t, first, name, who):
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _call(t, fn, *args):
-    """fn(*args, current stream) on t's device.  Where that is the current one already, as it nearly always is, the
-    context of torch.cuda.device and the stream object (3.5 us of a call of 10) are not needed."""
+# mxq_kv_call's numbers of the calls, and their arguments packed as it takes them (a double among the attention's)
+_TABLES, _APPEND, _READ, _ATTENTION = range(4)
+_tables_args, _append_args, _read_args = (struct.Struct("%dq" % n).pack for n in (17, 18, 10))
+_attention_args = struct.Struct("16qd8q").pack
+
+
+def _call(t, which, args, ws=None, ws_bytes=0):
+    """The call on t's device and its current stream.  Where that device is the current one already, as it nearly always
+    is, the context of torch.cuda.device and the stream object (3.5 us of a call of 10) are not needed."""
     index = t.get_device()
     if index >= 0 and index == _current_device():
-        rc = fn(*args, _raw_stream(index))
+        rc = _lib.gpu().mxq_kv_call(which, args, ws, ws_bytes, _raw_stream(index))
     else:
         with torch.cuda.device(t.device):
-            rc = fn(*args, _stream(t))
+            rc = _lib.gpu().mxq_kv_call(which, args, ws, ws_bytes, _stream(t))
     if rc != 0:
         _lib.check(rc, _lib.gpu())
 
@@ -171,10 +178,11 @@ def kv_block_tables(context_lens, new_lens, block_table, free_pages, free_start,
     ints = block_table.new_empty(2 * num_tokens + 2 * R + 2)
     positions, requests, starts, seq_lens, free_next = ints.split_with_sizes((num_tokens, num_tokens, R + 1, R, 1))
     first = ints.data_ptr()
-    _call(block_table, _lib.gpu().mxq_kv_block_tables, context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-          block_table.stride(0), table[1], free_pages.data_ptr(), free_pages.numel(), free_start.data_ptr(), R,
-          page_size, num_tokens, slots.data_ptr(), first, first + 4 * num_tokens, first + 8 * num_tokens,
-          first + 8 * num_tokens + 4 * (R + 1), first + 8 * num_tokens + 4 * (2 * R + 1))
+    _call(block_table, _TABLES, _tables_args(
+        context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), table[1],
+        free_pages.data_ptr(), free_pages.numel(), free_start.data_ptr(), R, page_size, num_tokens, slots.data_ptr(), first,
+        first + 4 * num_tokens, first + 8 * num_tokens, first + 8 * num_tokens + 4 * (R + 1),
+        first + 8 * num_tokens + 4 * (2 * R + 1)))
     return KVBlockTables(block_table, slots, positions, requests, starts, seq_lens, free_next)
 
 
@@ -213,9 +221,9 @@ def kv_append(cache, k, v, slots, scale_bits=8, round="nearest", flush_fp32_subn
             slots.is_contiguous() and round in _ROUNDINGS and not (k.requires_grad or v.requires_grad) and
             page_size % 16 == 0 and 16 <= page_size <= 65536 and 1 <= head_dim <= MAX_HEAD_DIM and shape[0] > 0 and shape[1] > 0):
         _check_append(cache, k, v, slots, round)
-    _call(data, _lib.gpu().mxq_kv_append_mx, k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], rows[0], ks[0], ks[1], vs[0], vs[1],
-          slots.data_ptr(), data.data_ptr(), shape[0], shape[1], page_size, head_dim, scale_bits,
-          1 if flush_fp32_subnorms else 0, _ROUNDINGS[round], _flags_value())
+    _call(data, _APPEND, _append_args(
+        k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], rows[0], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), data.data_ptr(),
+        shape[0], shape[1], page_size, head_dim, scale_bits, 1 if flush_fp32_subnorms else 0, _ROUNDINGS[round], _flags_value()))
 
 
 def kv_read(cache, slots, dtype=torch.float32):
@@ -234,8 +242,8 @@ def kv_read(cache, slots, dtype=torch.float32):
             raise RuntimeError("%s: Tensor dtype not supported (%s)" % (who, dtype))
     shape = (n[0], sizes[1], head_dim)
     k, v = data.new_empty(shape, dtype=dtype), data.new_empty(shape, dtype=dtype)
-    _call(data, _lib.gpu().mxq_kv_read_mx, k.data_ptr(), v.data_ptr(), _DTYPE[dtype], shape[0], slots.data_ptr(), data.data_ptr(),
-          sizes[0], sizes[1], page_size, head_dim)
+    _call(data, _READ, _read_args(k.data_ptr(), v.data_ptr(), _DTYPE[dtype], shape[0], slots.data_ptr(), data.data_ptr(), sizes[0],
+                                  sizes[1], page_size, head_dim))
     return k, v
 
 
@@ -305,12 +313,15 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
     rows, q_heads, width = q_shape[0], q_shape[1], table[1]
     lse = q.new_empty((rows, q_heads), dtype=torch.float32) if return_lse else None
     max_new = (1 if starts is None else rows) if max_new is None else max(1, int(max_new))
-    lib, dtype, outs = _lib.gpu(), _DTYPE[q.dtype], out.stride()
-    ws_bytes = lib.mxq_kv_attention_workspace_bytes(R, rows, q_heads, max_new, width, heads, page_size, head_dim, dtype)
-    ws = data.new_empty(ws_bytes) if ws_bytes else None
-    _call(data, lib.mxq_kv_attention_mx, q.data_ptr(), qs[0], qs[1], out.data_ptr(), outs[0], outs[1],
-          None if lse is None else lse.data_ptr(), dtype, rows, q_heads, block_table.data_ptr(), block_table.stride(0), width,
-          seq_lens.data_ptr(), None if starts is None else starts.data_ptr(), R, scale, 1 if causal else 0, max_new,
-          1 if new else 0, data.data_ptr(), shape[0], heads, page_size, head_dim, None if ws is None else ws.data_ptr(),
-          ws_bytes)
+    outs = out.stride()
+    args = _attention_args(
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), outs[0], outs[1], 0 if lse is None else lse.data_ptr(), _DTYPE[q.dtype], rows, q_heads,
+        block_table.data_ptr(), block_table.stride(0), width, seq_lens.data_ptr(), 0 if starts is None else starts.data_ptr(), R, scale,
+        1 if causal else 0, max_new, 1 if new else 0, data.data_ptr(), shape[0], heads, page_size, head_dim)
+    ws_bytes = _lib.gpu().mxq_kv_attention_args_workspace_bytes(args)
+    if ws_bytes:
+        ws = data.new_empty(ws_bytes)
+        _call(data, _ATTENTION, args, ws.data_ptr(), ws_bytes)
+    else:
+        _call(data, _ATTENTION, args)
     return (out, lse) if return_lse else out

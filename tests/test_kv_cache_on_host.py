@@ -17,7 +17,7 @@ UNITS = ("mxq_capi_kv.hip", "mxq_capi_kv_decode.hip", "mxq_capi_kv_prompt.hip")
 SKIP = "not stream and not captured and not 32_bits and not 290 and not workgroup_scans and not 600 and not fp16_rows"
 FEW = ("(append_then_read and (96 or 31)) or consecutive or layout or block_tables_of or (block_tables and (300 or 40)) or "
        "(single_tokens and (lens1 or lens7) and dtype0) or (single_tokens and lens5 and dtype1) or "
-       "(some_tokens and lens3) or (prompt_chunks and lens5) or missing_pages or (shared_by and lens0) or refusals or no_request or (not_in_order and starts0 and 60000) or "
+       "(some_tokens and lens3) or (prompt_chunks and lens5) or missing_pages or (shared_by and lens0) or refusals or in_an_array or no_request or (not_in_order and starts0 and 60000) or "
        "(wide_tables and lens3 and dtype0) or (wide_tables and lens6 and dtype1)")
 
 

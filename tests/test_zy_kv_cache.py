@@ -612,6 +612,15 @@ def test_refusals():
     assert torch.equal(before, s.cache.data)
 
 
+def test_calls_with_their_arguments_in_an_array():
+    lib = _lib.gpu()
+    for which in (-1, 4):
+        assert lib.mxq_kv_call(which, bytes(8 * 25), None, 0, None) != 0 and b"unknown call" in lib.mxq_last_error()
+    for which in range(4):                                        # zeros are refused by the calls themselves, before any launch
+        assert lib.mxq_kv_call(which, None, None, 0, None) != 0
+        assert lib.mxq_kv_call(which, bytes(8 * 25), None, 0, None) != 0
+
+
 # ---- the operators together ------------------------------------------------------------------------------------------
 def serve(steps, heads, group, dim, page, capture=False):
     """Requests grow step by step through tables, append and attention; every step's rows against the plain form."""
