@@ -779,7 +779,9 @@ struct KvShares {
 // number of its own, below rows G / (16 CT) + requests.
 __device__ __forceinline__ int kv_item(const KvAttnArgs& a, const KvSeq& s, int r) { return ((s.row0 * a.group) >> a.item_shift) + r; }
 
-// Waves that share a SIMD, from the registers of a wave: accumulators, q, the tile under way and the rest.
+// Waves that share a SIMD, from the registers of a wave: accumulators, q, the tile under way and the rest (as the compiler
+// needs them; 7 blocks, and 6 with fp16 queries, would spill at two waves).  More waves than fit lose more to spills than they
+// hide: 4 blocks at four waves 49.6 us instead of 41.8 (64 requests of 128 - 8192 tokens, 8 x 4 heads of 128).
 constexpr int kv_decode_registers(int nb, int ct, int terms) { return nb * (8 * ct + 4 * ct * terms + 7) + 72 + 18 * ct + 10 * (terms - 1); }
 constexpr int kv_decode_waves(int nb, int ct, int terms) {
     const int n = kv_decode_registers(nb, ct, terms);
