@@ -17,7 +17,7 @@ template <int DT>
 void launch_both_joins(const KvAttnArgs& a, const mxq_kv::Plan& p, hipStream_t s) {
     int64_t grid = a.join_blocks;
     MXQ_KV_CASES(p.nb,
-        if (p.prompt && (p.prompt_shares > 1 || !a.out_wide)) grid += p.prompt_items * a.c.heads * 4 * kv_prompt_ct(NB, kv_terms<DT>());
+        if (p.prompt && p.prompt_shares > 1) grid += p.prompt_items * a.c.heads * 4 * kv_prompt_ct(NB, kv_terms<DT>());
         if (grid > 0) kv_join_kernel<DT, NB><<<(unsigned)grid, kThreads, 0, s>>>(a))
 }
 

@@ -6,7 +6,10 @@ namespace {
 template <int DT>
 void launch(const KvAttnArgs& a, const mxq_kv::Plan& p, hipStream_t s) {
     const unsigned grid = (unsigned)(p.prompt_shares * a.c.heads);
-    MXQ_KV_CASES(p.nb, constexpr int CT = kv_prompt_ct(NB, kv_terms<DT>()); kv_prompt_kernel<DT, NB, CT><<<grid, kThreads, 0, s>>>(a))
+    MXQ_KV_CASES(p.nb,
+        constexpr int CT = kv_prompt_ct(NB, kv_terms<DT>());
+        if (a.out_wide) kv_prompt_kernel<DT, NB, CT, true><<<grid, kThreads, 0, s>>>(a);
+        else kv_prompt_kernel<DT, NB, CT, false><<<grid, kThreads, 0, s>>>(a))
 }
 
 }  // namespace

@@ -1000,7 +1000,7 @@ __device__ __forceinline__ void kv_prompt_join(const KvAttnArgs& a, int block) {
     const KvPlanView plan = kv_plan_view(a);
     if (plan.head[1] == 0 || item >= plan.head[0]) return;
     const int w0 = plan.items[2 * item], w1 = plan.items[2 * item + 1];
-    if (w0 == w1 && a.out_wide) return;
+    if (w0 == w1) return;                                // written by the workgroup that had all of it
     const KvPiece first = plan.pieces[item + w0];
     const int grp = first.group_flags >> 2;
     const KvSeq s = kv_seq(a, first.request);
@@ -1014,7 +1014,7 @@ __device__ __forceinline__ void kv_prompt_join(const KvAttnArgs& a, int block) {
         bool cut = false;
         for (int w = w0; w <= w1; ++w) {
             const KvPiece piece = plan.pieces[item + w];
-            if (piece.group_flags & 2 ? a.out_wide != 0 : piece.tile0 == piece.tile1) continue;   // written already; nothing done
+            if ((piece.group_flags & 2) || piece.tile0 == piece.tile1) continue;                  // written already; nothing done
             cut = true;
             const int64_t part = (((int64_t)w * a.c.heads + head) * 2 + (piece.group_flags & 1)) * COLS + col;
             const kv_f32x2 ml = *reinterpret_cast<const kv_f32x2*>(kv_prompt_part_ml<NB, COLS>(a, part));
@@ -1149,7 +1149,9 @@ struct KvShare {                                         // what a lane loads of
     uint32_t v[VB][2], vs[VB][2];                        // V: 32 tokens, every other block
 };
 
-template <int DT, int NB, int CT>
+// WIDE: a.out_wide.  (Decided while running, the stores of both kinds cost the loop scalar registers: 4001 tokens behind 12000,
+// 8 x 4 heads of 128, 1056 us instead of 1028.)
+template <int DT, int NB, int CT, bool WIDE>
 __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
     constexpr int NT = kv_terms<DT>(), NP = kv_terms<DT>(), COLS = 64 * CT, VB = KvShare<NB>::VB;
     using Wave = KvWave<NB, CT, NT, NP>;
@@ -1168,7 +1170,7 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
         const int r = uniform(piece.request), flags = uniform(piece.group_flags), grp = flags >> 2;
         const int tile0 = uniform(piece.tile0), tile1 = uniform(piece.tile1);
         if (tile0 == tile1 && !(flags & 2)) continue;
-        const bool complete = (flags & 2) && a.out_wide;        // (rows that are not aligned are the join kernel's)
+        const bool complete = (flags & 2) != 0;
         const KvSeq in_lanes = kv_seq(a, r);
         const KvSeq s{uniform(in_lanes.row0), uniform(in_lanes.fresh), uniform(in_lanes.len), uniform(in_lanes.keys)};
         const int columns = s.fresh * a.group;
@@ -1285,9 +1287,37 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
             }
             __syncthreads();
         }
-        if (!works) continue;
         // addresses below are worked out here: known before, they would be kept in registers through the loop above
         const int g_out = here_only(g4), i_out = here_only(i16);
+        if (!WIDE && complete) {
+            // Rows that are not aligned go through LDS, 16 columns of each wave at a time.  (As parts they would need a
+            // place for every item of the stretch; there are two, for the items that its ends cut.)
+            unsigned short* stage = reinterpret_cast<unsigned short*>(&s_k[0][0][0]) + wave * (16 * 32 * NB);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const float l = sum_over_groups(wv.l[ct]), inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const kv_f32x4 even = wv.acc[ct][b][0] * inv, odd = wv.acc[ct][b][1] * inv;
+                    *reinterpret_cast<u32x4*>(stage + i_out * (32 * NB) + 32 * b + 8 * g_out) =
+                        u32x4{Pack<DT>::put(even[0], odd[0]), Pack<DT>::put(even[1], odd[1]), Pack<DT>::put(even[2], odd[2]),
+                              Pack<DT>::put(even[3], odd[3])};
+                }
+                const int c = c0 + 16 * ct + i_out, token = a.by_group.of(c);
+                if (a.lse && g_out == 0 && c < columns)
+                    a.lse[(int64_t)(s.row0 + token) * a.c.heads * a.group + (int64_t)head * a.group + (c - token * a.group)] = kv_lse(wv.m[ct], l);
+                __syncthreads();
+#pragma nounroll
+                for (int e = here_only(lane); e < 16 * 32 * NB; e += 64) {
+                    const int x = c0 + 16 * ct + e / (32 * NB), d = e % (32 * NB), t = a.by_group.of(x);
+                    if (x < columns && d < a.c.head_dim)
+                        kv_out_row(a, s.row0 + t, (int64_t)head * a.group + (x - t * a.group))[d] = stage[e];
+                }
+                __syncthreads();                             // what is there has been read
+            }
+            continue;
+        }
+        if (!works) continue;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             const float l = sum_over_groups(wv.l[ct]);

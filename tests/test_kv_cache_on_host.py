@@ -69,3 +69,23 @@ def test_gpu_tests_pass_on_the_kernels_compiled_for_the_host(host_build):
     assert res.returncode == 0, tail
     assert " passed" in res.stdout and "failed" not in res.stdout, tail
     print(tail)
+
+
+# of the edges, what takes a minute or two; behind the skipped ones are prompts of thousands of rows
+EDGES = "(several_items_in_a_stretch and lens0 and dtype0)"
+EDGES_SKIP = "not long_prompts"
+
+
+def test_edges_pass_on_the_kernels_compiled_for_the_host(host_build):
+    if os.environ.get("MXQ_KERNELS_ON_HOST") == "none":
+        pytest.skip("MXQ_KERNELS_ON_HOST=none")
+    select = EDGES_SKIP if os.environ.get("MXQ_KERNELS_ON_HOST") == "all" else "(%s) and %s" % (EDGES, EDGES_SKIP)
+    env = dict(os.environ, MXQ_HIP_ON_HOST_LIB=host_build,
+               PYTHONPATH=os.path.join(ROOT_DIR, "tests") + os.pathsep + os.environ.get("PYTHONPATH", ""))
+    res = subprocess.run([sys.executable, "-m", "pytest", "-p", "hip_on_host_plugin", "-p", "no:cacheprovider", "-q", "-x",
+                          "-m", "gpu", "-k", select, "--durations=8", "tests/test_zy_kv_cache_edges.py"],
+                         cwd=ROOT_DIR, env=env, capture_output=True, text=True, timeout=2 * 3600)
+    tail = res.stdout[-6000:] + res.stderr[-2000:]
+    assert res.returncode == 0, tail
+    assert " passed" in res.stdout and "failed" not in res.stdout, tail
+    print(tail)

@@ -1,0 +1,87 @@
+"""The packed key / value cache at its edges: what the shapes of test_zy_kv_cache.py, whose Setup and tolerances serve here
+too, do not reach."""
+import math
+
+import pytest
+import torch
+
+from microxcaling_amd import _lib
+from microxcaling_amd import custom_extensions as ce
+from microxcaling_amd.kv_cache import kv_append, kv_attention, kv_read, new_kv_cache
+from test_zy_kv_cache import DEV, Setup, gen, takes_prompt_kernel
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- prompt chunks whose output rows are not 16-byte aligned, several items in a workgroup's stretch --------------------
+# 64 kv heads of more than 6 blocks share the prompt kernel's 256 workgroups: four stretches a head, and an item has 64
+# columns (16 query heads a kv head: four rows).  So 40 rows are 10 items, and two stretches hold an item from its first
+# tile to its last between parts of two others.
+SEVERAL = [([40], [40], 64, 16, 225, 16, True), ([33, 33, 33, 33], [8, 9, 10, 11], 64, 16, 230, 16, True),
+           ([60], [40], 64, 16, 241, 48, False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,new,heads,group,dim,page,causal", SEVERAL)
+def test_rows_of_any_length_with_several_items_in_a_stretch(lens, new, heads, group, dim, page, causal, dtype):
+    s = Setup(lens, new, heads, group, dim, page, dtype, seed=30, spare=50)
+    assert takes_prompt_kernel(s, max(new))
+    s.check(s.call(max_new=max(new), causal=causal), causal=causal, terms=1 if dtype == torch.bfloat16 else 2)
+
+
+def test_given_outputs_that_are_not_aligned_with_several_items_in_a_stretch():
+    s = Setup([40], [40], 64, 16, 256, 16, seed=31, spare=50)
+    assert takes_prompt_kernel(s, 40)
+    out = torch.full((40, 1024, 264), 7.0, dtype=s.q.dtype, device=DEV)
+    got = s.call(max_new=40, out=out[:, :, 3:259])
+    s.check(got, terms=1)
+    assert (out[:, :, :3] == 7).all() and (out[:, :, 259:] == 7).all()
+    want = s.call(max_new=40)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def attention_in_64_bits(q, k, v, scale):
+    """(out, lse, a bound on what a kernel may be off by: Setup.want's, with the probabilities as one bf16 term) of one
+    request whose rows are its last tokens; k, v as the cache holds them."""
+    n, new, H = k.shape[0], q.shape[0], k.shape[1]
+    G = q.shape[1] // H
+    hidden = torch.arange(n, device=q.device)[None] > torch.arange(n - new, n, device=q.device)[:, None]
+    outs, lses, tols, ltols = [], [], [], []
+    for h in range(H):
+        kh, vh = k[:, h].double(), v[:, h].double()
+        for g in range(h * G, h * G + G):
+            x = q[:, g].double()
+            z = (x @ kh.T * scale).masked_fill_(hidden, -math.inf)
+            lse = z.logsumexp(-1)
+            top = z.masked_fill_(hidden, 0).abs().amax(-1)
+            off = (k.shape[2] + 4) * 2.0 ** -24 * (x.abs() @ kh.abs().T * abs(scale)).amax(-1) + 2.0 ** -22 * (1 + top)
+            p = (z - lse[:, None]).exp_().masked_fill_(hidden, 0)
+            out = p @ vh
+            part = 2 * off + (n + 16) * 2.0 ** -24 + 2.0 ** -8
+            outs.append(out)
+            lses.append(lse)
+            tols.append(torch.finfo(q.dtype).eps / 2 * out.abs() * (1 + 2.0 ** -7) + part[:, None] * (p @ vh.abs()) + 1e-30)
+            ltols.append(off + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * lse.abs())
+    return (torch.stack(t, 1) for t in (outs, lses, tols, ltols))
+
+
+@pytest.mark.parametrize("context,new,heads,group,dim,page", [(0, 2048, 8, 4, 100, 16), (700, 4001, 8, 4, 100, 64), (0, 4096, 32, 1, 127, 32)])
+def test_long_prompts_with_rows_of_any_length(context, new, heads, group, dim, page):
+    """Hundreds of rows in a stretch, at sizes of ordinary prompts (their fp64 result is worked out on the GPU)."""
+    n = context + new
+    g = torch.Generator(DEV).manual_seed(32)
+    k, v = (torch.randn(n, heads, dim, generator=g, device=DEV).bfloat16() for _ in range(2))
+    q = torch.randn(new, heads * group, dim, generator=g, device=DEV).bfloat16()
+    pages = -(-n // page)
+    cache = new_kv_cache(pages + 1, page, heads, dim, DEV)
+    table = torch.randperm(pages + 1, generator=gen(33))[None, :pages].int().to(DEV)
+    t = torch.arange(n, device=DEV)
+    slots = table[0].long()[t // page] * page + t % page
+    kv_append(cache, k, v, slots)
+    lens, starts = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([n], [0, new]))
+    want, lse, tol, ltol = attention_in_64_bits(q, *kv_read(cache, slots), dim ** -0.5)
+    wide = torch.empty(new, heads * group, dim + 9, dtype=q.dtype, device=DEV)
+    for out in (None, wide[:, :, 5:5 + dim]):
+        got, got_lse = kv_attention(q, cache, table, lens, starts, max_new=new, out=out, return_lse=True)
+        assert ((got.double() - want).abs() <= tol).all()
+        assert ((got_lse.double() - lse).abs() <= ltol).all()
