@@ -812,7 +812,8 @@ void kv_decode_kernel(KvAttnArgs a) {
         head_rows = head_rows < 0 ? 0 : (head_rows < rows ? head_rows : rows);
         tail = tail < head_rows ? head_rows : (tail < rows ? tail : rows);
         const int heads = a.c.heads * a.group, nobodys = (head_rows + rows - tail) * heads;
-        for (uint32_t x = blockIdx.x; x < (uint32_t)nobodys; x += gridDim.x) {   // (rows x heads and the grid: below 2^31 each)
+        const uint32_t workgroups = gridDim.x - (a.plan ? 1u : 0u);          // (kv_plan's has left)
+        for (uint32_t x = blockIdx.x; x < (uint32_t)nobodys; x += workgroups) {  // (rows x heads and the grid: below 2^31 each)
             const int e = (int)x < head_rows * heads ? (int)x : (int)x + (tail - head_rows) * heads;
             unsigned short* o = kv_out_row(a, e / heads, e % heads);
             if (a.zero_tail)

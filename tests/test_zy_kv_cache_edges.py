@@ -8,7 +8,7 @@ import torch
 from microxcaling_amd import _lib
 from microxcaling_amd import custom_extensions as ce
 from microxcaling_amd.kv_cache import kv_append, kv_attention, kv_read, new_kv_cache
-from test_zy_kv_cache import DEV, Setup, gen, takes_prompt_kernel
+from test_zy_kv_cache import DEV, Setup, gen, takes_prompt_kernel, wide_table
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,37 @@ def test_long_prompts_with_rows_of_any_length(context, new, heads, group, dim, p
         got, got_lse = kv_attention(q, cache, table, lens, starts, max_new=new, out=out, return_lse=True)
         assert ((got.double() - want).abs() <= tol).all()
         assert ((got_lse.double() - lse).abs() <= ltol).all()
+
+
+# ---- rows of no request, more of them than the decode kernel has workgroups -----------------------------------------------
+def call_into(s, q, out, lse, hint, zero_tail=1, starts=None):
+    """The C call with buffers that hold something already."""
+    lib, table, seq = _lib.gpu(), s.table.to(DEV), s.seq.to(DEV)
+    st = (s.starts if starts is None else starts).to(DEV)
+    rows, heads = q.shape[0], q.shape[1]
+    need = lib.mxq_kv_attention_workspace_bytes(len(s.lens), rows, heads, hint, table.shape[1], s.heads, s.page, s.dim, ce._DTYPE[q.dtype])
+    ws = torch.full((need,), 0xA5, dtype=torch.uint8, device=DEV)
+    data = s.cache.data
+    rc = lib.mxq_kv_attention_mx(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+                                 ce._DTYPE[q.dtype], rows, heads, table.data_ptr(), table.stride(0), table.shape[1], seq.data_ptr(),
+                                 st.data_ptr(), len(s.lens), s.dim ** -0.5, 1, hint, zero_tail, data.data_ptr(), data.shape[0], s.heads,
+                                 s.page, s.dim, ws.data_ptr(), need, None)
+    _lib.check(rc, lib)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new,heads,group,dim,before,behind", [(80, 1, 4, 32, 0, 400), (70, 8, 4, 128, 37, 60), (40, 8, 4, 256, 1, 200)])
+def test_many_rows_of_no_request_beside_prompt_chunks(new, heads, group, dim, before, behind):
+    s = Setup([new], [new], heads, group, dim, 16, seed=34, spare=wide_table([new], heads * group, 16))
+    assert takes_prompt_kernel(s, new)
+    rows, q_heads = before + new + behind, heads * group
+    q = torch.full((rows, q_heads, dim), math.nan, dtype=s.q.dtype)
+    q[before:before + new] = s.q
+    nobody = torch.ones(rows, dtype=torch.bool)
+    nobody[before:before + new] = False
+    for zero_tail in (1, 0):
+        out, lse = torch.full((rows, q_heads, dim), 7.0, dtype=s.q.dtype, device=DEV), torch.full((rows, q_heads), 7.0, device=DEV)
+        call_into(s, q.to(DEV), out, lse, new, zero_tail, s.starts + before)
+        assert (out.cpu()[nobody] == (0 if zero_tail else 7)).all()
+        assert (lse.cpu()[nobody] == -math.inf).all()
+        s.check((out[before:before + new], lse[before:before + new]), terms=1)
