@@ -84,7 +84,8 @@ def _check_on(t, first, name, who):
         raise RuntimeError("%s: %s is on %s, not on %s" % (who, name, t.device, first.device))
 
 
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# (a torch without GPU support lacks the two; its tensors are refused before a call gets to them)
+_current_device, _raw_stream = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 
 
 # mxq_kv_call's numbers of the calls, and their arguments packed as it takes them (a double among the attention's)

@@ -370,3 +370,22 @@ def test_the_written_notes_name_things_that_exist():
             if name not in sources:
                 missing.append((doc, name))
     assert not missing, missing
+
+
+def test_the_package_works_on_a_torch_without_gpu_support():
+    """Such a build lacks torch._C._cuda_*: the import and the CPU path do without them."""
+    import subprocess
+    import sys
+    from helpers import ROOT_DIR
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, n)\n"
+            "assert not torch.cuda.is_available()\n"
+            "import microxcaling_amd as mx\n"
+            "from microxcaling_amd.mx_ops import _quantize_mx\n"
+            "y = _quantize_mx(torch.arange(64.0).view(2, 32), 8, 'fp4_e2m1', axes=[-1], block_size=32)\n"
+            "assert y[0, 31] == 24 and y[1, 31] == 48, y\n"
+            "try: mx.kv_read(mx.new_kv_cache(1, 16, 1, 32, 'cpu'), torch.zeros(1, dtype=torch.int64))\n"
+            "except RuntimeError as e: assert 'CUDA tensor' in str(e), e\n"
+            "else: assert False\n")
+    res = subprocess.run([sys.executable, "-c", code], cwd=ROOT_DIR, capture_output=True, text=True, timeout=600)
+    assert res.returncode == 0, res.stderr
