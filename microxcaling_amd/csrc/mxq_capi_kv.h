@@ -5,6 +5,9 @@
 #include "mxq_kv_attention.h"
 
 namespace mxq_kv {
+// workgroups of a launch: its threads are counted in 32 bits, and what is above them is left out without an error
+constexpr int64_t kMostWorkgroups = 0xFFFFFFFF / kThreads;
+
 // what a call of the attention runs
 struct Plan {
     int nb, ct;                    // blocks of a row; column tiles of a decode item

@@ -77,7 +77,7 @@ Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64
     // A workgroup for each item, and no join: 32 requests of 500, 760, 1000, 1500 tokens (8 x 4 heads of 128) 11.3, 13.7, 16.3,
     // 20.7 us, against 16.6, 17.0, 19.3, 21.8 with the units dealt out; 8 requests 12.2, 13.9, 17.7 against 13.0, 13.9, 14.9
     // from 760 on; one request 10.5, 12.1, 13.7 against 11.5, 11.7, 11.7.
-    p.whole = units <= 4 || (units <= 8 && requests * heads >= 64);
+    p.whole = (units <= 4 || (units <= 8 && requests * heads >= 64)) && p.decode_items * heads < mxq_kv::kMostWorkgroups;
     const int64_t chip = 256 * kv_decode_waves(nb, p.ct, terms);
     p.shares = ceil_div(chip, heads) < KV_MAX_SHARES ? ceil_div(chip, heads) : KV_MAX_SHARES;
     if (p.shares > p.decode_items * units) p.shares = p.decode_items * units;
@@ -236,8 +236,9 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     const int64_t needed = part_bytes(p, heads, terms, requests);
     // units and items are numbered in 32 bits
     const int64_t most_units = (requests + ceil_div(rows * q_heads / heads, 16)) * (ceil_div(width * page_size, KV_UNIT) + 1 + KV_ITEM_UNITS);
-    // .. and so are the workgroups of a launch
-    if (most_units > 0x7FFFFFFF || p.prompt_items * heads * 16 + (int64_t)128 * requests * heads > 0x7FFFFFFF || p.decode_items * heads > 0x7FFFFFFF) return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
+    // .. and so are the join's workgroups
+    const int64_t most_joins = p.prompt ? p.prompt_items * heads * 16 + (int64_t)128 * requests * heads : rows * q_heads;
+    if (most_units > 0x7FFFFFFF || most_joins > 0x7FFFFFFF) return fail(MXQ_ERR_ARGUMENT, "%s: size too large", who);
     if (workspace_bytes < needed || (needed > 0 && !workspace))
         return fail(MXQ_ERR_ARGUMENT, "%s: the workspace is too small", who);
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(MXQ_ERR_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
@@ -284,6 +285,7 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     // requests with few columns have few rows where the others are the prompt kernel's
     const int64_t join = p.whole ? 0 : (p.prompt ? a.join_rows * requests : rows) * q_heads;
     a.join_blocks = (int)join;
+    a.join_first = 0;
     hipStream_t s = (hipStream_t)hip_stream;
     mxq_kv::launch_decode(dtype, &a, p, s);
     if ((rc = check_launch(who))) return rc;

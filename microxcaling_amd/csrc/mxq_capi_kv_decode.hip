@@ -18,7 +18,12 @@ void launch_both_joins(const KvAttnArgs& a, const mxq_kv::Plan& p, hipStream_t s
     int64_t grid = a.join_blocks;
     MXQ_KV_CASES(p.nb,
         if (p.prompt && p.prompt_shares > 1) grid += p.prompt_items * a.c.heads * 4 * kv_prompt_ct(NB, kv_terms<DT>());
-        if (grid > 0) kv_join_kernel<DT, NB><<<(unsigned)grid, kThreads, 0, s>>>(a))
+        KvAttnArgs part = a;
+        for (int64_t first = 0; first < grid; first += mxq_kv::kMostWorkgroups) {
+            const int64_t rest = grid - first;
+            part.join_first = (int)first;
+            kv_join_kernel<DT, NB><<<(unsigned)(rest < mxq_kv::kMostWorkgroups ? rest : mxq_kv::kMostWorkgroups), kThreads, 0, s>>>(part);
+        })
 }
 
 }  // namespace

@@ -52,6 +52,7 @@ struct KvAttnArgs {
     int* spans;                                          // decode: where the parts of each item lie (two numbers, KvShares)
     float* part;                                         // decode: partial results, two places for each workgroup
     int join_blocks;                                     // join: workgroups for decode rows, the others for prompt items
+    int join_first;                                      // join: the first workgroup of this launch
     int prompt_shares, prompt_items;                     // prompt: workgroups of a kv head and items of it, at most
     float* prompt_part;
     void* plan;                                          // null: no prompt kernel
@@ -1053,13 +1054,14 @@ __global__ __launch_bounds__(TPB) void kv_join_kernel(KvAttnArgs a) {
     __shared__ float s_weight[KV_MAX_SHARES];
     __shared__ float s_top[TPB / 64], s_sum[TPB / 64];
     __shared__ kv_f32x4 s_acc[ROWS][LANES];
-    if ((int)blockIdx.x >= a.join_blocks) {
-        kv_prompt_join<DT, NB, kv_prompt_ct(NB, kv_terms<DT>())>(a, (int)blockIdx.x - a.join_blocks);
+    const int block = a.join_first + (int)blockIdx.x;
+    if (block >= a.join_blocks) {
+        kv_prompt_join<DT, NB, kv_prompt_ct(NB, kv_terms<DT>())>(a, block - a.join_blocks);
         return;
     }
     const int q_heads = a.c.heads * a.group;
-    int64_t row = a.by_q_heads.of(blockIdx.x);
-    const int qh = (int)blockIdx.x - (int)row * q_heads, head = a.by_group.of(qh);
+    int64_t row = a.by_q_heads.of(block);
+    const int qh = block - (int)row * q_heads, head = a.by_group.of(qh);
     int r = (int)row;
     if (a.join_rows) {                                   // the first rows of each request: others are the prompt kernel's
         r = (int)(row / a.join_rows);

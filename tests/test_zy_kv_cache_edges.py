@@ -119,3 +119,38 @@ def test_many_rows_of_no_request_beside_prompt_chunks(new, heads, group, dim, be
         assert (out.cpu()[nobody] == (0 if zero_tail else 7)).all()
         assert (lse.cpu()[nobody] == -math.inf).all()
         s.check((out[before:before + new], lse[before:before + new]), terms=1)
+
+
+# ---- more rows and heads than a launch has workgroups (2^32 threads of 256 a workgroup) -----------------------------------
+@pytest.mark.parametrize("rows,heads,group,width,long", [(132000, 1, 128, 65, 600), (131500, 128, 1, 1, 0)])
+def test_more_rows_than_a_launch_has_workgroups(rows, heads, group, width, long):
+    """Requests that share their pages, most of them short; the last ones, beyond the first launch of the join, long
+    enough to be cut.  Or (width 1) more items than workgroups that take a whole one."""
+    dim, page = 1, 16
+    g = torch.Generator(DEV).manual_seed(35)
+    cache = new_kv_cache(width, page, heads, dim, DEV)
+    slots = torch.arange(width * page, device=DEV)
+    kv_append(cache, *(torch.randn(width * page, heads, dim, generator=g, device=DEV).bfloat16() for _ in range(2)), slots)
+    k, v = (t.double()[..., 0] for t in kv_read(cache, slots))                       # (tokens, heads)
+    lens = torch.randint(0, 6, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    lens[rows - long:] = width * page - 3
+    q = torch.randn(rows, heads * group, dim, generator=g, device=DEV).bfloat16()
+    table = torch.arange(width, dtype=torch.int32, device=DEV).expand(rows, width).contiguous()
+    out, lse = kv_attention(q, cache, table, lens, scale=0.7, out=torch.full_like(q, 7.0), return_lse=True)
+    for r0, r1 in ((0, rows - long), (rows - long, rows)):
+        n = int(lens[r0:r1].max()) if r1 > r0 else 0
+        for a in range(r0, r1, 20000):
+            b = min(a + 20000, r1)
+            z = q[a:b].double().view(b - a, heads, group, 1) * k[:n].T[None, :, None] * 0.7
+            z = z.masked_fill(torch.arange(n, device=DEV) >= lens[a:b, None, None, None], -math.inf)
+            want_lse = z.logsumexp(-1)
+            p = torch.where(torch.isfinite(want_lse)[..., None], (z - want_lse[..., None]).exp(), 0.0)
+            want, weight = ((p * x[:n].T[None, :, None]).sum(-1).view(b - a, -1, 1) for x in (v, v.abs()))
+            top = z.masked_fill(z == -math.inf, 0).abs().amax(-1)
+            off = (dim + 4) * 2.0 ** -24 * top + 2.0 ** -22 * (1 + top)
+            tol = 2.0 ** -8 * want.abs() * (1 + 2.0 ** -7) + (2 * off.view(b - a, -1, 1) + (n + 16) * 2.0 ** -24 + 2.0 ** -16) * weight + 1e-30
+            assert ((out[a:b].double() - want).abs() <= tol).all()
+            want_lse = want_lse.view(b - a, -1)
+            assert torch.equal(torch.isinf(lse[a:b]), torch.isinf(want_lse))
+            near = (lse[a:b].double() - want_lse).abs() <= off.view(b - a, -1) + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * want_lse.abs()
+            assert (near | torch.isinf(want_lse)).all()
