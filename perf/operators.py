@@ -217,7 +217,7 @@ def prepare(case, seed):
         pages = int(sum(-(-(int(h) + int(n)) // S) for h, n in zip(held.tolist(), fresh.tolist()))) + 5
         table, order, used = _tables_of(held, S, width, pages, gen, device)
         free = order[used:].contiguous()
-        return dict(state, rows=_rows(case), held=held.int(), fresh=fresh.int(), table=table, free=free,
+        return dict(state, held=held.int(), fresh=fresh.int(), table=table, free=free,
                     free_start=torch.zeros(1, dtype=torch.int32, device=device))
     H, G, D = case["heads"], case["group"], case["dim"]
     pages = int(sum(-(-(int(h) + int(n)) // S) for h, n in zip(held.tolist(), fresh.tolist()))) + 2
@@ -238,7 +238,7 @@ def prepare(case, seed):
 # ---- one pass --------------------------------------------------------------------------------------------------------
 def _plain_tables(s):
     held, fresh, table, free, S = s["held"].long(), s["fresh"].long(), s["table"], s["free"], s["case"]["page"]
-    R, width, rows = held.numel(), table.shape[1], s["rows"]
+    R, width, rows = held.numel(), table.shape[1], _rows(s["case"])
     first, last = (held + S - 1) // S, ((held + fresh + S - 1) // S).clamp(max=width)
     need = (last - first).clamp(min=0)
     from_ = s["free_start"].long() + need.cumsum(0) - need
@@ -333,7 +333,7 @@ def run(state):
     case = state["case"]
     if op == "tables":
         t = kv_cache.kv_block_tables(state["held"], state["fresh"], state["table"], state["free"], state["free_start"],
-                                     case["page"], state["rows"])
+                                     case["page"], _rows(case))
         return {"table": t.block_table, "slots": t.slots, "positions": t.positions, "requests": t.requests,
                 "starts": t.starts, "seq_lens": t.seq_lens, "free_start": t.free_start}
     cache = kv_cache.PackedKVCache(state["data"], case["page"], case["dim"])
