@@ -200,21 +200,35 @@ __device__ __forceinline__ void kv_v_operands(const uint32_t codes[2], const uin
 }
 
 // The V scales of a masked tile of 32 tokens (t0 ..; a lane: tokens 4 g + r of halves j): tokens behind `end` or on
-// missing pages and tokens whose block is NaN get the scale 2^-127, since even a probability of 0 times NaN is NaN.
-// Returns which of the 32 tokens have a NaN block; their columns are told by kv_spread_nan.
-__device__ __forceinline__ uint32_t kv_mend_scales(uint32_t scales[2], const bool there[2], int t0, int g, int end) {
-    uint32_t nan = 0;
+// missing pages and elements that are NaN or Inf get the scale 2^-127, since even a probability of 0 times one of them is NaN.
+// Returns in which of the 32 tokens the block has such an element; their columns are told by spread_nan.  (A code of 2^2 and
+// more times 2^126, or of 2 and more times 2^127, is Inf: the quantizer gets there with bf16 values from 2^127 * 1.75 on.)
+__device__ __forceinline__ uint32_t kv_mend_scales(uint32_t scales[2], const uint32_t codes[2], const bool there[2], int t0, int g,
+                                                   int end) {
+    uint32_t high = 0;                                   // has a byte from 253 on
     g = here_only(g);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (!(there[j] && t0 + 16 * j + 4 * g + r < end)) scales[j] &= ~(255u << (8 * r));
+        high |= ((scales[j] & 0x7F7F7F7Fu) + 0x03030303u) & scales[j] & 0x80808080u;
+    }
+    if (!any_lane(high != 0u)) return 0;
+    uint32_t bad = 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const bool seen = there[j] && t0 + 16 * j + 4 * g + r < end;
-            const bool is_nan = ((scales[j] >> (8 * r)) & 255u) == 255u;
-            if (is_nan && seen) nan |= 1u << (16 * j + 4 * g + r);
-            if (is_nan || !seen) scales[j] &= ~(255u << (8 * r));
+            const uint32_t scale = (scales[j] >> (8 * r)) & 255u, pair = codes[j] >> (8 * r);
+            const uint32_t least = scale == 255u ? 0u : scale == 254u ? 4u : 6u;
+            if (scale >= 253u && ((pair & 7u) >= least || ((pair >> 4) & 7u) >= least)) {
+                bad |= 1u << (16 * j + 4 * g + r);
+                scales[j] &= ~(255u << (8 * r));
+            }
         }
-    return nan;
+    for (int d = 1; d < 16; d <<= 1) bad |= (uint32_t)__shfl_xor((int)bad, d, 64);           // (a lane has two elements of the block)
+    return or_over_groups(bad);
 }
 
 // Eight 16-bit elements e0 .. of a row that ends at `end`, where rows are not aligned.  A loop, not unrolled: unrolled,
@@ -433,7 +447,7 @@ struct KvWave {
         }
     }
 
-    // block b is NaN in the tokens `of` (of 32 from t0): so is it in the columns that see one of them
+    // block b has NaN or Inf in the tokens `of` (of 32 from t0): it is NaN in the columns that see one of them
     __device__ __forceinline__ void spread_nan(int b, uint32_t of, int t0) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
@@ -557,12 +571,13 @@ struct KvWave {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 uint32_t scales[2] = {values.vs[0][b], values.vs[1][b]};
-                nan_of[b] = kv_mend_scales(scales, there, t0, g, max_limit);
+                const uint32_t codes[2] = {values.v[0][b], values.v[1][b]};
+                nan_of[b] = kv_mend_scales(scales, codes, there, t0, g, max_limit);
                 values.vs[0][b] = scales[0];
                 values.vs[1][b] = scales[1];
                 all |= nan_of[b];
             }
-            any_nan = any_lane(all != 0u);
+            any_nan = uniform((int)all) != 0;
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -575,7 +590,7 @@ struct KvWave {
         fetch_values(a, values, p, after);
         if (any_nan) {                                   // rare
 #pragma unroll
-            for (int b = 0; b < NB; ++b) spread_nan(b, or_over_groups(nan_of[b]), t0);
+            for (int b = 0; b < NB; ++b) spread_nan(b, nan_of[b], t0);
         }
     }
 };
@@ -1232,11 +1247,11 @@ __global__ __launch_bounds__(TPB, 2) void kv_prompt_kernel(KvAttnArgs a) {
                 const int b = (wave >> 1) + 2 * x;
                 if (b < NB) {
                     uint32_t scales[2] = {share.vs[x][0], share.vs[x][1]};
+                    const uint32_t codes[2] = {share.v[x][0], share.v[x][1]};
                     if (masked) {
-                        const uint32_t nan = or_over_groups(kv_mend_scales(scales, there2, 64 * tile + 32 * half, g4, wg_max));
+                        const uint32_t nan = kv_mend_scales(scales, codes, there2, 64 * tile + 32 * half, g4, wg_max);
                         if (lane == 0) s_nan[buffer][half][b] = nan;
                     }
-                    const uint32_t codes[2] = {share.v[x][0], share.v[x][1]};
                     kv_bf16x8 v8[2];
                     kv_v_operands(codes, scales, v8);
 #pragma unroll

@@ -286,7 +286,8 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
     seq_lens (int32): tokens of each request, the new ones (already appended) included.  starts (int32, requests + 1):
     request r has the rows starts[r] .. starts[r + 1] - 1, which are its last tokens; None: one row a request.  With
     causal a row sees the tokens up to its own, otherwise all of its request.  Tokens whose page is not in the cache are
-    not seen.  A row that sees no token gets zeros (lse -inf).  Rows of no request (before the first one's and behind the
+    not seen.  NaN or Inf in the cache reaches the rows that see its token (in a value: some or all of its block of 32), no
+    others.  A row that sees no token gets zeros (lse -inf).  Rows of no request (before the first one's and behind the
     last one's) are zero in a new output and left as they are in a given `out`; their lse is -inf.  scale defaults to
     head_dim ** -0.5.
 

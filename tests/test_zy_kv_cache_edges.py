@@ -154,3 +154,30 @@ def test_more_rows_than_a_launch_has_workgroups(rows, heads, group, width, long)
             assert torch.equal(torch.isinf(lse[a:b]), torch.isinf(want_lse))
             near = (lse[a:b].double() - want_lse).abs() <= off.view(b - a, -1) + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * want_lse.abs()
             assert (near | torch.isinf(want_lse)).all()
+
+
+# ---- values whose rounding overflows -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("prompt,dim,lens,new,at", [(False, 64, [40], [30], 21), (False, 128, [70, 33], [1, 1], 20), (True, 64, [180], [170], 41),
+                                                    (True, 160, [150], [140], 130)])
+def test_a_value_that_overflows_reaches_the_rows_that_see_it_only(prompt, dim, lens, new, at, dtype):
+    """3.3e38 is rounded to 4 * 2^126, which is Inf, as quantize_mx has it.  Rows before the token are untouched, and so are
+    the other blocks of the rows that see it."""
+    runs = []
+    for bad in (False, True):
+        s = Setup(lens, new, 1, 2, dim, 16, dtype, seed=36, spare=wide_table(new, 2, 16) if prompt else 0)
+        assert takes_prompt_kernel(s, max(new)) == prompt
+        if bad:
+            s.v[0][at, 0, 37] = 3.3e38
+            kv_append(s.cache, s.k[0].to(DEV), s.v[0].to(DEV), s.slots[0].to(DEV))
+            assert kv_read(s.cache, s.slots[0][at:at + 1].to(DEV))[1][0, 0, 37] == math.inf
+        runs.append([t.cpu() for t in s.call(max_new=max(new))])
+    (want, want_lse), (out, lse) = runs
+    first = max(0, at - (lens[0] - new[0]))                       # the first row that sees the token
+    last = new[0]
+    assert torch.equal(lse, want_lse)
+    assert torch.equal(out[:first], want[:first]) and torch.equal(out[last:], want[last:])
+    assert not torch.isfinite(out[first:last, :, 37]).any()
+    others = torch.ones(dim, dtype=torch.bool)
+    others[32:64] = False
+    assert torch.equal(out[..., others], want[..., others])
