@@ -274,8 +274,11 @@ def _check_attention(q, cache, block_table, seq_lens, starts, out):
         _check_on(out, data, "out", who)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise RuntimeError("%s: out must be %s %s, got %s %s" % (who, q.dtype, tuple(q.shape), out.dtype, tuple(out.shape)))
-        if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-            raise RuntimeError("%s: rows of out share memory" % who)
+        reach = 1                                        # from the narrowest stride to the widest: each passes what is inside it
+        for step, n in sorted((step, n) for n, step in zip(out.shape, out.stride()) if n > 1):
+            if step < reach:
+                raise RuntimeError("%s: rows of out share memory" % who)
+            reach += step * (n - 1)
 
 
 def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causal=True, max_new=None, out=None,
@@ -289,7 +292,7 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
     not seen.  NaN or Inf in the cache reaches the rows that see its token (in a value: some or all of its block of 32), no
     others.  A row that sees no token gets zeros (lse -inf).  Rows of no request (before the first one's and behind the
     last one's) are zero in a new output and left as they are in a given `out`; their lse is -inf.  scale defaults to
-    head_dim ** -0.5.
+    head_dim ** -0.5.  out may be q itself, but may not overlap it, or itself, in another way.
 
     max_new: the most rows that a request has, if known: it steers the choice of kernels, never the result.  return_lse:
     also the logarithm of the sum of exponentials, fp32 (rows, query heads).  Accumulation, maxima and sums are fp32; the

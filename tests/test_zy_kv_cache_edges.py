@@ -181,3 +181,27 @@ def test_a_value_that_overflows_reaches_the_rows_that_see_it_only(prompt, dim, l
     others = torch.ones(dim, dtype=torch.bool)
     others[32:64] = False
     assert torch.equal(out[..., others], want[..., others])
+
+
+# ---- given outputs -------------------------------------------------------------------------------------------------------
+def test_outputs_whose_rows_overlap_are_refused():
+    s = Setup([20, 20], [1, 1], 2, 2, 64, 16)
+    room = torch.zeros(2 * 4 * 64, dtype=s.q.dtype, device=DEV)
+    for strides in ((256, 32, 1), (64, 64, 1), (1, 64, 1), (255, 64, 1), (0, 64, 1)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            s.call(single=True, out=room.as_strided((2, 4, 64), strides))
+    want = s.call(single=True)
+    for out in (room.view(4, 2, 64).transpose(0, 1), room.as_strided((2, 4, 64), (256, 64, 1)), torch.zeros(4, 3, 70, dtype=s.q.dtype, device=DEV)[:, :2, 1:65].transpose(0, 1)):
+        got = s.call(single=True, out=out)
+        assert got[0] is out and torch.equal(out, want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("lens,new,heads,group,dim,spare", [([33, 0, 7], [1, 1, 1], 2, 4, 128, 0), ([700, 30], [3, 5], 1, 4, 64, 60), ([90, 33], [80, 33], 1, 4, 64, 6000),
+                                                           ([90, 33], [80, 33], 1, 4, 66, 6000)])
+def test_the_queries_as_output(lens, new, heads, group, dim, spare):
+    """Every result replaces the query it belongs to: one workgroup, shared-out requests, the prompt kernel."""
+    s = Setup(lens, new, heads, group, dim, 16, seed=37, spare=spare)
+    assert takes_prompt_kernel(s, max(new)) == (spare == 6000)
+    want, q = s.call(max_new=max(new)), s.q.to(DEV)
+    got = s.call(q=q, max_new=max(new), out=q)
+    assert got[0] is q and torch.equal(q, want[0]) and torch.equal(got[1], want[1])
