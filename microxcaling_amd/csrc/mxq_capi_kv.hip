@@ -223,7 +223,8 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     if (q_heads < 1 || q_heads % heads != 0)
         return fail(MXQ_ERR_ARGUMENT, "%s: %d query heads do not share %d kv heads evenly", who, q_heads, heads);
     if (rows < 0 || requests < 0 || width < 0) return fail(MXQ_ERR_ARGUMENT, "%s: negative size", who);
-    if (!(scale > -__builtin_inff() && scale < __builtin_inff())) return fail(MXQ_ERR_ARGUMENT, "%s: scale must be finite", who);
+    const float scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
+    if (!(scale_log2 < __builtin_inff())) return fail(MXQ_ERR_ARGUMENT, "%s: scale must be finite, also times log2(e)", who);
     if (rows == 0) return MXQ_OK;
     if (requests == 0 && !starts) return fail(MXQ_ERR_ARGUMENT, "%s: rows without requests", who);
     if (!starts && rows != requests) return fail(MXQ_ERR_ARGUMENT, "%s: without starts every request has one row", who);
@@ -260,7 +261,7 @@ int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.by_heads = kv_divide((uint32_t)heads);
     a.by_q_heads = kv_divide((uint32_t)q_heads);
     a.rows = rows;
-    a.scale_log2 = (scale < 0 ? -scale : scale) * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     if (a.scale_log2 < 1.17549435e-38f) a.scale_log2 = 1.17549435e-38f;      // 0 times a masked score of -inf would be NaN
     a.negative = scale < 0 ? 1 : 0;
     a.causal = causal ? 1 : 0;

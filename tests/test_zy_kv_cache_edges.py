@@ -205,3 +205,12 @@ def test_the_queries_as_output(lens, new, heads, group, dim, spare):
     want, q = s.call(max_new=max(new)), s.q.to(DEV)
     got = s.call(q=q, max_new=max(new), out=q)
     assert got[0] is q and torch.equal(q, want[0]) and torch.equal(got[1], want[1])
+
+
+def test_scales_that_are_too_large_are_refused():
+    """Scores are taken to base 2: |scale| * log2(e) has to be an fp32 number too."""
+    s = Setup([20, 20], [1, 1], 2, 2, 64, 16)
+    for scale in (2.4e38, -2.4e38, 3.4e38, 1e39, -math.inf):
+        with pytest.raises(RuntimeError, match="scale"):
+            s.call(single=True, scale=scale)
+    s.check(s.call(single=True, scale=100.0), scale=100.0)
