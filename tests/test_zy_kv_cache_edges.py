@@ -214,3 +214,28 @@ def test_scales_that_are_too_large_are_refused():
         with pytest.raises(RuntimeError, match="scale"):
             s.call(single=True, scale=scale)
     s.check(s.call(single=True, scale=100.0), scale=100.0)
+
+
+# ---- several rows a request in the decode kernel, whose probabilities are two bf16 terms ----------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,new,heads,group,dim,page,causal,hint", [
+    ([100, 35, 0, 64], [70, 1, 0, 64], 2, 2, 64, 16, True, 70), ([150], [101], 1, 4, 128, 48, True, 101), ([140], [130], 1, 1, 80, 16, True, 130),
+    ([90, 77], [70, 77], 1, 1, 256, 16, True, 77), ([90], [35], 1, 3, 96, 32, False, 35), ([80], [80], 1, 1, 33, 16, True, 80),
+    ([81], [66], 1, 2, 200, 16, True, 66), ([40, 19, 64], [3, 1, 5], 1, 4, 64, 16, True, None), ([130, 9], [9, 9], 1, 6, 96, 48, False, 1),
+    ([20, 5], [2, 7], 1, 3, 32, 16, True, None), ([700, 90], [9, 40], 2, 2, 64, 16, True, 4)])
+def test_chunks_in_the_decode_kernel_keep_both_terms(lens, new, heads, group, dim, page, causal, hint, dtype):
+    """Within 2^-16 of each probability: one term alone is off by up to 2^-8."""
+    s = Setup(lens, new, heads, group, dim, page, dtype, seed=38, spare=40 if max(lens) == 700 else 0)
+    assert not takes_prompt_kernel(s, sum(new) if hint is None else hint)
+    s.check(s.call(causal=causal, max_new=hint), causal=causal, terms=2)
+
+
+@pytest.mark.parametrize("new", [2, 40])
+def test_missing_pages_in_the_decode_kernel_keep_both_terms(new):
+    s = Setup([100, 64, 50], [new] * 3, 1, 2, 64, 16, seed=39)
+    assert not takes_prompt_kernel(s, new)
+    s.table[0, 2], s.table[0, 4], s.table[1] = -1, 2 ** 31 - 1, s.cache.data.shape[0]
+    missing = torch.zeros(100, dtype=torch.bool)
+    missing[32:48] = missing[64:80] = True
+    seen = {0: ~missing, 1: torch.zeros(64, dtype=torch.bool), 2: torch.ones(50, dtype=torch.bool)}
+    s.check(s.call(max_new=new), seen=lambda r: seen[r], terms=2)
