@@ -239,3 +239,47 @@ def test_missing_pages_in_the_decode_kernel_keep_both_terms(new):
     missing[32:48] = missing[64:80] = True
     seen = {0: ~missing, 1: torch.zeros(64, dtype=torch.bool), 2: torch.ones(50, dtype=torch.bool)}
     s.check(s.call(max_new=new), seen=lambda r: seen[r], terms=2)
+
+
+# ---- the prompt kernel, its plan and its parts in graphs and on streams ----------------------------------------------------
+def test_captured_prompt_chunks_replay_with_new_lengths():
+    """Two graphs over the same cache, aligned and unaligned rows, padding behind; lengths and starts change in place and the
+    program's own calls come between the replays."""
+    s = Setup([300, 260], [200, 150], 2, 4, 72, 16, seed=40, spare=wide_table([360], 8, 16))
+    assert takes_prompt_kernel(s, 200)
+    table, seq, starts = s.table.to(DEV), s.seq.to(DEV), s.starts.to(DEV)
+    qs = [torch.randn(400, 8, 72, generator=gen(seed)).bfloat16().to(DEV) for seed in (41, 42)]
+    call = lambda n: kv_attention(qs[n], s.cache, table, seq, starts, max_new=200, return_lse=True,
+                                  out=None if n == 0 else torch.zeros(400, 8, 80, dtype=torch.bfloat16, device=DEV)[:, :, 3:75])
+    call(0), call(1)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for n in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(n))
+        graphs.append(graph)
+    for step in range(6):
+        seq.copy_(torch.tensor([[300, 260], [200, 7], [1, 260]][step % 3], dtype=torch.int32))
+        starts.copy_(torch.tensor([[0, 200, 350], [0, 200, 200], [3, 3, 160]][step % 3], dtype=torch.int32))
+        graphs[step % 2].replay()
+        got = [t.clone() for t in outs[step % 2]]
+        torch.cuda.synchronize()
+        for a, b in zip(got, call(step % 2)):
+            assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once():
+    sets = [Setup([300, 260], [200, 150], 2, 4, 72, 16, seed=43, spare=wide_table([350], 8, 16)),
+            Setup([900, 45, 2000], [1, 3, 2], 2, 4, 128, 16, seed=44, spare=60)]
+    args = [(s.q.to(DEV), s.cache, s.table.to(DEV), s.seq.to(DEV), s.starts.to(DEV)) for s in sets]
+    want = [kv_attention(*a, max_new=max(s.new), return_lse=True) for a, s in zip(args, sets)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for _ in range(10):
+        for n, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append((n, kv_attention(*args[n], max_new=max(sets[n].new), return_lse=True)))
+    torch.cuda.synchronize()
+    for n, (out, lse) in got:
+        assert torch.equal(out, want[n][0]) and torch.equal(lse, want[n][1])
