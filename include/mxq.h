@@ -363,8 +363,10 @@ int mxq_kv_read_mx(void* k, void* v, int dtype, int64_t tokens, const int64_t* s
  * h / (q_heads / heads).  Request r's rows are starts[r] .. starts[r + 1] - 1 (starts NULL: row r), the last of its
  * seq_lens[r] tokens; with causal a row sees the tokens up to its own.  Tokens on pages that do not exist are not
  * seen; a row that sees nothing gets zeros and lse -inf.  Rows of no request are left as they are, or
- * zeroed with zero_tail; their lse is -inf.  max_new: the most rows of a request, a hint that only steers the choice of
- * kernels.  workspace: mxq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned. */
+ * zeroed with zero_tail; their lse is -inf.  NaN or Inf in the cache reaches the rows that see its token, no others.
+ * max_new: the most rows of a request, a hint.  The result is right whatever it is, but it and the table's width choose the
+ * kernels, and bits and error are theirs (probabilities as two bf16 terms, or as one for large chunks of bf16 queries).
+ * scale times log2(e) has to be finite in fp32.  out may be q, but may not overlap it in another way.  workspace: mxq_kv_attention_workspace_bytes(...) bytes, 16-byte aligned. */
 int mxq_kv_attention_mx(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
                         int64_t out_head_stride, float* lse, int dtype, int64_t rows, int q_heads, const int* block_table,
                         int64_t table_stride, int64_t width, const int* seq_lens, const int* starts, int64_t requests,

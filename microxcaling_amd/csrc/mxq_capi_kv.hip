@@ -55,7 +55,8 @@ int rows_grid(const KvCache& c, int64_t tokens) {
 }
 
 // Which kernels a call runs, and with what shares.  max_new: tokens that a request brings at most (a hint: every
-// choice made with it is right for any number).
+// choice made with it is right for any number).  room: tokens that a table row can name.  It stands for the lengths, which
+// the host does not know: short prompts in wide tables take the prompt kernel too.  What is measured here is bf16.
 Plan make_plan(int64_t requests, int64_t rows, int group, int64_t max_new, int64_t room, int heads, int nb, int terms) {
     Plan p;
     p.nb = nb;

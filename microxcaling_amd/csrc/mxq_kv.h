@@ -33,7 +33,8 @@ typedef __bf16 kv_bf16x2 __attribute__((ext_vector_type(2)));
 constexpr int KV_MAX_NB = 8;                             // head_dim up to 256
 constexpr int KV_TOKEN_BYTES = 34;                       // bytes of a token's K and V for each block of 32
 
-// Division of 32-bit numbers by one that the host knows: five instructions instead of forty.
+// Division of 32-bit numbers by one that the host knows (Granlund and Montgomery, Division by Invariant Integers using
+// Multiplication, 1994): five instructions instead of forty.
 struct KvDivide {
     uint32_t by, first, then;                            // n / d = (h + (n - h >> first)) >> then, h = high half of n by
     __device__ __forceinline__ uint32_t of(uint32_t n) const {

@@ -12,9 +12,9 @@
 // Sums, maxima and accumulators are fp32.
 //
 // What bounds it, measured at 8 kv heads of 128 with 4 query heads each: reading the cache for single tokens (64 requests of
-// 128 - 8192 tokens, 135 MB: 34.5 us, 5.6 TB/s while the waves walk; 131072 + 2048 tokens 32.8 us), instruction issue for
-// prompts (4001 tokens behind 12000: 1.0 ms, 890 TFLOP/s, matrix instructions 37 % and vector instructions 47 % of
-// the cycles).  A tile of 32 tokens costs 276 vector instructions, 64 of them conversions from fp4.  The 4-bit scaled matrix
+// 128 - 8192 tokens, 135 MB: 33.4 us, 5.6 TB/s while the waves walk; 131072 + 2048 tokens 31.8 us), instruction issue for
+// prompts (4001 tokens behind 12000: a call 1.00 ms, 917 TFLOP/s, matrix instructions 39 % and vector instructions 47 %
+// of the cycles).  A tile of 32 tokens costs 257 vector instructions, 64 of them conversions from fp4.  The 4-bit scaled matrix
 // instruction, which would take K as it lies, is not used: its sums are off by 2^-13.5 of their absolute terms.
 //
 // Two kernels share this body.  kv_decode_kernel (few columns): the waves of a workgroup take turns over the

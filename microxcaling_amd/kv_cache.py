@@ -294,9 +294,10 @@ def kv_attention(q, cache, block_table, seq_lens, starts=None, scale=None, causa
     last one's) are zero in a new output and left as they are in a given `out`; their lse is -inf.  scale defaults to
     head_dim ** -0.5.  out may be q itself, but may not overlap it, or itself, in another way.
 
-    max_new: the most rows that a request has, if known: it steers the choice of kernels, never the result.  return_lse:
-    also the logarithm of the sum of exponentials, fp32 (rows, query heads).  Accumulation, maxima and sums are fp32; the
-    probabilities enter the second product as two bf16 terms, or as one for large chunks of bf16 queries."""
+    max_new: the most rows that a request has, if known.  A hint: the result is right whatever it is, but it and the table's
+    width choose the kernels, and bits and error are theirs.  Accumulation, maxima and sums are fp32 in all of them.  The
+    probabilities enter the second product as two bf16 terms (off by up to 2^-17 of each); in the kernel for large chunks with
+    bf16 queries as one (2^-8).  return_lse: also the logarithm of the sum of exponentials, fp32 (rows, query heads)."""
     data, page_size, head_dim = cache
     at, shape, table, q_shape, R = data.get_device(), data.shape, block_table.shape, q.shape, seq_lens.numel()
     qs, heads = q.stride(), shape[1] if len(shape) == 3 else 0
